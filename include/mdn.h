@@ -476,6 +476,115 @@ int mdn_gae_normalize_static(const float* rewards, const float* values, const fl
                              float* returns, uint32_t horizon, uint32_t envs, float gamma, float lambda,
                              void* stream);
 
+/* ---- memory block (no reference counterpart) --------------------------- */
+/* Operators of a policy with a recurrent memory, for callers that own their
+ * device buffers (a torch program through the Python veneer, or plain CUDA):
+ * like mdn_gae_normalize_static they take device pointers and a stream
+ * (cudaStream_t, NULL = the default stream), allocate nothing and do not
+ * synchronise, so they may be captured into a CUDA graph. They run on the
+ * current device. Arrays are time-major like the rollout buffers and carry
+ * their own strides, so that slices of a fused projection are taken as they
+ * are. Several calls may run at once on different streams as long as they do
+ * not share output, workspace or saved buffers. */
+#define MDN_F32 0u
+#define MDN_BF16 1u
+
+/* A [steps][envs][heads][dim] array: strides in elements, dim contiguous.
+ * Decays and betas are [steps][envs][heads] (no dim axis). */
+typedef struct mdn_rows {
+    void* data;
+    int64_t step, env, head;
+} mdn_rows;
+
+/* The gated delta rule: per environment and head a memory S [key][value],
+ *   S <- exp(log_decay_t) S        (S <- 0 first where starts_t is set)
+ *   u_t = beta_t (v_t - S^T k_t),  S <- S + k_t u_t^T,  out_t = scale S^T q_t.
+ * With MDN_DELTA_NORMALIZE q_t and k_t are first divided by
+ * sqrt(|x|^2 + norm_eps). Value heads share query/key heads in groups:
+ * head h uses q/k head h / (heads / qk_heads). Products are accumulated and
+ * states kept in 32 bits whatever dtype is. */
+#define MDN_DELTA_NORMALIZE 1u
+#define MDN_DELTA_MAX_DIM 128u
+typedef struct mdn_delta {
+    uint32_t steps, envs, heads, qk_heads;
+    uint32_t key_dim, value_dim;     /* 1..MDN_DELTA_MAX_DIM                          */
+    uint32_t dtype;                  /* MDN_F32 / MDN_BF16: q, k, v, out and gradients */
+    uint32_t flags;                  /* MDN_DELTA_*                                   */
+    float scale, norm_eps;
+    mdn_rows q, k, v;                /* q, k: qk_heads heads of key_dim; v: heads of value_dim */
+    mdn_rows log_decay, beta;        /* float; log_decay <= 0 is the caller's to keep */
+    const uint8_t* starts;           /* NULL, or [steps][envs]: an episode starts at this step */
+    int64_t starts_step, starts_env;
+    const int32_t* lengths;          /* NULL, or [envs]: steps at and past lengths[env] are not
+                                        read; their outputs and gradients are zeros and the
+                                        state stays as it is                          */
+    const float* state_in;           /* [envs][heads][key][value]; NULL = zeros. Not read for an
+                                        environment whose first step is a start       */
+    float* state_out;                /* the same shape; may be state_in; NULL = not wanted     */
+    mdn_rows out;                    /* heads of value_dim                            */
+    void* saved;                     /* NULL, or what the gradients need from this call:
+                                        mdn_delta_saved_bytes bytes, 16-byte aligned  */
+} mdn_delta;
+
+typedef struct mdn_delta_grads {
+    mdn_rows dout;                   /* in: gradient of out                           */
+    const float* dstate_out;         /* in: gradient of state_out; NULL = zeros       */
+    mdn_rows dq, dk, dv;             /* out, in dtype (qk_heads / qk_heads / heads)   */
+    mdn_rows dlog_decay, dbeta;      /* out, float                                    */
+    float* dstate_in;                /* out; NULL = not wanted                        */
+    void* workspace;                 /* mdn_delta_workspace_bytes bytes, 16-byte aligned; may be
+                                        NULL when that is 0                           */
+} mdn_delta_grads;
+
+/* Sizes for a call's shape (only its shape fields are read); 0 on a bad shape. */
+size_t mdn_delta_saved_bytes(const mdn_delta* call);
+size_t mdn_delta_workspace_bytes(const mdn_delta* call);
+/* One rollout (any number of steps, 0 and 1 among them: one step is the
+ * policy tick). steps, envs of 0 are allowed. */
+int mdn_delta_forward(const mdn_delta* call, void* stream);
+/* Its gradients. `call` as it was given to mdn_delta_forward, with `saved`
+ * filled by that call; its out and state_out are not read. Deterministic:
+ * sums over a group's heads are taken in a fixed order. */
+int mdn_delta_backward(const mdn_delta* call, const mdn_delta_grads* grads, void* stream);
+
+/* The norms around a block, fused with its gate and residual scale:
+ *   h = x + residual_scale * act(gate) * (branch / rms(branch) * branch_weight)
+ *   y = h / rms(h) * norm_weight,       rms(r) = sqrt(mean r^2 + eps)
+ * over rows of `dim` values: the norm after one block and the norm before the
+ * next in one pass. branch NULL: h = x (not written), the norm before the
+ * first block; gate NULL: act = 1; a weight or scale NULL: 1; y NULL: only h.
+ * x, h: stream_dtype; branch, gate, y: dtype; weights float. Row strides in
+ * elements, values contiguous. Statistics and sums in 32 bits; y is computed
+ * from h before h is rounded. */
+#define MDN_GATE_SIGMOID 0u
+#define MDN_GATE_SILU 1u
+#define MDN_NORM_MAX_DIM 8192u
+typedef struct mdn_matrix {
+    void* data;
+    int64_t row;
+} mdn_matrix;
+typedef struct mdn_block_norm {
+    uint64_t rows;
+    uint32_t dim, dtype, stream_dtype, gate_act;
+    float eps;
+    mdn_matrix x, branch, gate;
+    const float *branch_weight, *residual_scale, *norm_weight;
+    mdn_matrix h, y;
+} mdn_block_norm;
+/* Gradients, from h as it was written (rounded to stream_dtype). dh NULL or dy
+ * NULL: zeros. Outputs whose input was NULL are not written; other NULL
+ * outputs are not wanted. Weight gradients are sums over all rows in a fixed
+ * order (deterministic). */
+typedef struct mdn_block_norm_grads {
+    mdn_matrix dh, dy;                                       /* in  */
+    mdn_matrix dx, dbranch, dgate;                           /* out */
+    float *dbranch_weight, *dresidual_scale, *dnorm_weight;  /* out, [dim] */
+    void* workspace;     /* mdn_block_norm_workspace_bytes bytes, 16-byte aligned */
+} mdn_block_norm_grads;
+size_t mdn_block_norm_workspace_bytes(const mdn_block_norm* call);
+int mdn_block_norm_forward(const mdn_block_norm* call, void* stream);
+int mdn_block_norm_backward(const mdn_block_norm* call, const mdn_block_norm_grads* grads, void* stream);
+
 /* ---- deployment export ----------------------------------------------- */
 /* Write a trained actor in the reference's deployable format: NAVPOL1 for the
  * 64-unit actor (nav_deployment::NavigationPolicy::write_file,

@@ -14,6 +14,20 @@ from .capi import (ChallengeBank, ChallengeSampler, Device, MdnError, PPOTrainer
                    checkpoint_inspect, default_raptor, evaluate_bank, gather_rollout_evidence, lib, runtime_config,
                    sha256_file, task_control, task_settings, write_policy)
 
+# The operators on torch tensors (memory.py) are loaded on first use, so that the
+# rest of the package does not import torch.
+_MEMORY = ("DeltaSaved", "block_norm", "block_norm_backward", "block_norm_train", "delta_rule", "delta_rule_backward",
+           "delta_rule_train", "delta_step")
+
+
+def __getattr__(name):
+    if name not in _MEMORY:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import memory
+    globals().update((n, getattr(memory, n)) for n in _MEMORY)
+    return globals()[name]
+
+
 PACKAGE_DIR = pathlib.Path(__file__).resolve().parent
 
 

@@ -89,6 +89,13 @@ SIGNATURES = {
     "mdn_ppo_checkpoint_load": (ctypes.c_int, [_P, ctypes.c_char_p, _U, _U, _U, _U]),
     "mdn_gae_normalize_static": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _U, _U, ctypes.c_float,
                                                  ctypes.c_float, _P]),
+    "mdn_delta_saved_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
+    "mdn_delta_workspace_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
+    "mdn_delta_forward": (ctypes.c_int, [ctypes.c_char_p, _P]),
+    "mdn_delta_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _P]),
+    "mdn_block_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
+    "mdn_block_norm_forward": (ctypes.c_int, [ctypes.c_char_p, _P]),
+    "mdn_block_norm_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _P]),
     "mdn_sim_set_challenge_bank": (ctypes.c_int, [_P, _P, _P]),
     "mdn_domain_stress_range": (None, [_P]),
     "mdn_sim_set_runtime": (ctypes.c_int, [_P, _P]),
