@@ -17,7 +17,6 @@ namespace mdn {
 namespace {
 
 constexpr int kCell = 16;  // steps between two saved states
-constexpr int kThreads = 128;
 
 using bf16 = __nv_bfloat16;
 
@@ -33,35 +32,10 @@ __device__ __forceinline__ T* row_ptr(const mdn_rows& r, uint32_t t, uint32_t en
     return static_cast<T*>(r.data) + int64_t(t) * r.step + int64_t(env) * r.env + int64_t(head) * r.head;
 }
 
-__device__ __forceinline__ float block_sum(float x, float* scratch) {
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-    __syncthreads();
-    float sum = 0.0f;
-    for (int w = 0; w < kThreads / 32; w++) sum += scratch[w];
-    return sum;
-}
-
 __device__ __forceinline__ uint32_t live_steps(const mdn_delta& c, uint32_t env) {
     if (!c.lengths) return c.steps;
     const int32_t n = c.lengths[env];
     return n <= 0 ? 0u : min(uint32_t(n), c.steps);
-}
-
-// One step's key or query row into shared memory, divided by its length when
-// the call asks for it; returns the factor.
-template <class T>
-__device__ __forceinline__ float load_row(const mdn_delta& c, const mdn_rows& rows, uint32_t t, uint32_t env,
-                                          uint32_t head, float* dst, float* scratch) {
-    const T* p = row_ptr<T>(rows, t, env, head);
-    const float x = threadIdx.x < c.key_dim ? to_float(p[threadIdx.x]) : 0.0f;
-    float r = 1.0f;
-    if (c.flags & MDN_DELTA_NORMALIZE) r = 1.0f / sqrtf(block_sum(x * x, scratch) + c.norm_eps);
-    __syncthreads();
-    if (threadIdx.x < c.key_dim) dst[threadIdx.x] = x * r;
-    __syncthreads();
-    return r;
 }
 
 // ------------------------------------------------------------------ tick
@@ -201,7 +175,7 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) k_delta_tick(const __grid
 //
 // Precision: the tensor cores multiply bf16. A 32-bit value is cut into three
 // bf16 parts of 8 significant bits each, which hold it exactly, and products
-// of parts i and j are taken where i + j <= 2: what is left out is below 2^-24
+// of parts i and j are taken where i + j <= 2: what is left out is about 2^-25
 // of the product. bf16 inputs are one exact part.
 //
 // A warp holds 16 value columns of the state, S^T as the accumulator layout of
@@ -231,12 +205,20 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The next 8 significant bits of x and y as a packed bf16 pair, cut off x and y.
+// x and y to the nearest bf16 as a packed pair.
+__device__ __forceinline__ uint32_t round_pair(float x, float y) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+// The same, and x and y become what is left: three times over holds them
+// exactly. Rounded rather than cut off, so that what a product leaves out has
+// no common sign.
 __device__ __forceinline__ uint32_t cut(float& x, float& y) {
-    const uint32_t xi = __float_as_uint(x), yi = __float_as_uint(y);
-    x -= __uint_as_float(xi & 0xffff0000u);
-    y -= __uint_as_float(yi & 0xffff0000u);
-    return __byte_perm(xi, yi, 0x7632);
+    const uint32_t r = round_pair(x, y);
+    x -= __uint_as_float(r << 16);
+    y -= __uint_as_float(r & 0xffff0000u);
+    return r;
 }
 // Two accumulator tiles (16 rows x 16 columns) as the N parts of an A operand.
 template <int N>
@@ -253,6 +235,43 @@ __device__ __forceinline__ void mma_parts(float (&d0)[4], float (&d1)[4], const 
                                           const uint32_t (&b)[NB][4]) {
 #pragma unroll
     for (int order = 2; order >= 0; order--)
+#pragma unroll
+        for (int i = 0; i < NA; i++) {
+            const int j = order - i;
+            if (j < 0 || j >= NB) continue;
+            mma(d0, a[i], b[j][0], b[j][1]);
+            mma(d1, a[i], b[j][2], b[j][3]);
+        }
+}
+
+// The same with the small products (order 1 and 2) in accumulators of their
+// own: the tensor cores round every accumulation toward zero, which over
+// several k steps costs bits where large and small products share a sum.
+template <int NA, int NB>
+__device__ __forceinline__ void mma_parts(float (&d0)[4], float (&d1)[4], float (&e0)[4], float (&e1)[4],
+                                          const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
+#pragma unroll
+    for (int order = 2; order >= 1; order--)
+#pragma unroll
+        for (int i = 0; i < NA; i++) {
+            const int j = order - i;
+            if (j < 0 || j >= NB) continue;
+            mma(e0, a[i], b[j][0], b[j][1]);
+            mma(e1, a[i], b[j][2], b[j][3]);
+        }
+    mma(d0, a[0], b[0][0], b[0][1]);
+    mma(d1, a[0], b[0][2], b[0][3]);
+}
+
+// For a result that is stored as bf16 the operands have two parts and the
+// product of both second parts is left out: 2^-18 where the store rounds at 2^-9;
+// with three parts all products count.
+template <int NA, int NB>
+__device__ __forceinline__ void mma_out(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
+                                        const uint32_t (&b)[NB][4]) {
+    constexpr int last = NA == 3 && NB == 3 ? 2 : NA == 2 || NB == 2 ? 1 : 2;
+#pragma unroll
+    for (int order = last; order >= 0; order--)
 #pragma unroll
         for (int i = 0; i < NA; i++) {
             const int j = order - i;
@@ -286,7 +305,7 @@ __device__ __forceinline__ void cp_async_wait() {
 struct ChunkMeta {
     uint32_t t, n;      // first step, steps (0: the rollout is done)
     uint32_t fresh;     // an episode starts at t
-    uint32_t slot;      // where its rows are
+    uint32_t unused;
 };
 
 // Walks a rollout's chunks in order: cells of 16 steps, cut at episode starts.
@@ -326,29 +345,31 @@ struct ChunkWalk {
     }
 };
 
-// `count` rows of `dim` values from step t on into shared rows of `row`
-// bytes, `width` values wide; what lies past `dim` or past the rows is zeros.
-template <class T>
+// n <= 16 rows of `dim` values from step t on into shared rows of ROW bytes,
+// WIDTH values wide; what lies past `dim` or past the rows is zeros.
+template <class T, int WIDTH, int ROW>
 __device__ __forceinline__ void fetch_rows(const mdn_rows& src, bool vec, uint32_t t, uint32_t env, uint32_t head,
-                                           uint32_t first, uint32_t dim, uint32_t n, char* dst, uint32_t row,
-                                           uint32_t width, uint32_t lane) {
+                                           uint32_t first, uint32_t dim, uint32_t n, char* dst, uint32_t lane) {
     const T* base = row_ptr<T>(src, t, env, head) + first;
-    constexpr uint32_t per = 16 / sizeof(T);
     if (vec) {
-        const uint32_t granules = width / per;  // a power of two
-        const uint32_t shift = 31 - __clz(granules);
-        for (uint32_t e = lane; e < kCell * granules; e += 32) {
-            const uint32_t r = e >> shift, col = (e & (granules - 1)) * per;
-            const uint32_t values = r < n && col < dim ? min(per, dim - col) : 0;
-            cp_async16(smem_addr(dst + r * row + col * sizeof(T)), values ? base + int64_t(r) * src.step + col : base,
-                       values * sizeof(T));
+        constexpr uint32_t per = 16 / sizeof(T), granules = WIDTH / per, rows = 32 / granules;
+        const uint32_t r0 = lane / granules, col = lane % granules * per;
+        const uint32_t bytes = col < dim ? min(per, dim - col) * uint32_t(sizeof(T)) : 0u;
+        const T* p = base + int64_t(r0) * src.step + col;
+        uint32_t d = smem_addr(dst) + r0 * ROW + lane % granules * 16;
+#pragma unroll
+        for (uint32_t r = 0; r < kCell; r += rows) {
+            const uint32_t got = r0 + r < n ? bytes : 0u;
+            cp_async16(d, got ? p : base, got);
+            p += rows * src.step;
+            d += rows * ROW;
         }
     } else {
-        for (uint32_t e = lane; e < kCell * width; e += 32) {
-            const uint32_t r = e / width, col = e % width;
+        for (uint32_t e = lane; e < kCell * WIDTH; e += 32) {
+            const uint32_t r = e / WIDTH, col = e % WIDTH;
             T x = T(0.0f);
             if (r < n && col < dim) x = base[int64_t(r) * src.step + col];
-            *reinterpret_cast<T*>(dst + r * row + col * sizeof(T)) = x;
+            *reinterpret_cast<T*>(dst + r * ROW + col * sizeof(T)) = x;
         }
     }
 }
@@ -379,169 +400,204 @@ __device__ __forceinline__ void cut_rows(const char* raw, uint32_t raw_row, char
     }
 }
 
-// Sum of squares of the row that two lanes share (lane / 2), in both.
-template <class T, int DK>
+// Sum of squares of the 32-bit row that two lanes share (lane / 2), in both.
+template <int DK>
 __device__ __forceinline__ float row_squares(const char* raw, uint32_t raw_row, uint32_t lane) {
-    const T* p = reinterpret_cast<const T*>(raw + (lane >> 1) * raw_row) + (lane & 1) * (DK / 2);
-    float sum = 0.0f;
+    const float* p = reinterpret_cast<const float*>(raw + (lane >> 1) * raw_row) + (lane & 1) * (DK / 2);
+    float sum[4] = {};
 #pragma unroll
-    for (int i = 0; i < DK / 2; i += 16 / int(sizeof(T))) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p + i);
-        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if constexpr (sizeof(T) == 4) {
-                const float v = __uint_as_float(x[e]);
-                sum = fmaf(v, v, sum);
-            } else {
-                const float lo = __uint_as_float(x[e] << 16), hi = __uint_as_float(x[e] & 0xffff0000u);
-                sum = fmaf(lo, lo, sum);
-                sum = fmaf(hi, hi, sum);
-            }
-        }
+    for (int i = 0; i < DK / 2; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p + i);
+        sum[0] = fmaf(x.x, x.x, sum[0]), sum[1] = fmaf(x.y, x.y, sum[1]);
+        sum[2] = fmaf(x.z, x.z, sum[2]), sum[3] = fmaf(x.w, x.w, sum[3]);
     }
-    return sum + __shfl_xor_sync(~0u, sum, 1);
+    const float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    return s + __shfl_xor_sync(~0u, s, 1);
 }
 
+__device__ __forceinline__ void load16(float (&x)[16], const float* p) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(p + i);
+        x[i] = y.x, x[i + 1] = y.y, x[i + 2] = y.z, x[i + 3] = y.w;
+    }
+}
+
+// k_j.k_i and k_j.q_i of a chunk's steps as [j][i], and |q_j|^2 where the
+// inputs are single bf16 parts (`squares`).
+template <int NP, int DK, int ROW>
+__device__ __forceinline__ void key_products(const char* keys, const char* queries, float* kk, float* kq,
+                                             float* squares, uint32_t lane) {
+    const uint32_t g = lane >> 2, t = lane & 3, qp = smem_addr(queries), kp = smem_addr(keys);
+    float dk0[4] = {}, dk1[4] = {}, dq0[4] = {}, dq1[4] = {}, qq0[4] = {}, qq1[4] = {};
+#pragma unroll
+    for (int kb = 0; kb < DK / 16; kb++) {
+        uint32_t ak[NP][4], bk[NP][4], bq[NP][4];
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            ldsm4(ak[p], kp + p * kCell * ROW + kb * 32 + lane_rows_first(lane, ROW));
+            ldsm4(bq[p], qp + p * kCell * ROW + kb * 32 + lane_cols_first(lane, ROW));
+            // the same blocks in the other order
+            bk[p][0] = ak[p][0], bk[p][1] = ak[p][2], bk[p][2] = ak[p][1], bk[p][3] = ak[p][3];
+        }
+        mma_parts<NP, NP>(dk0, dk1, ak, bk);
+        mma_parts<NP, NP>(dq0, dq1, ak, bq);
+        if constexpr (NP == 1) {
+            const uint32_t aq[4] = {bq[0][0], bq[0][2], bq[0][1], bq[0][3]};
+            mma(qq0, aq, bq[0][0], bq[0][1]);
+            mma(qq1, aq, bq[0][2], bq[0][3]);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t at = (g + 8 * h) * kScratchRow + 2 * t;
+        *reinterpret_cast<float2*>(kk + at) = make_float2(dk0[2 * h], dk0[2 * h + 1]);
+        *reinterpret_cast<float2*>(kk + at + 8) = make_float2(dk1[2 * h], dk1[2 * h + 1]);
+        *reinterpret_cast<float2*>(kq + at) = make_float2(dq0[2 * h], dq0[2 * h + 1]);
+        *reinterpret_cast<float2*>(kq + at + 8) = make_float2(dq1[2 * h], dq1[2 * h + 1]);
+    }
+    if (NP == 1 && t == g >> 1) {
+        squares[g] = g & 1 ? qq0[1] : qq0[0];
+        squares[8 + g] = g & 1 ? qq1[3] : qq1[2];
+    }
+}
+
+// 1 / sqrt(x), the hardware's estimate with a Newton step.
+__device__ __forceinline__ float unit_factor(float x) {
+    const float r = rsqrtf(x);
+    return x > 0.0f && r > 0.0f ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
+}
+
+// Column j of (I + A)^-1 by forward substitution, each step's value subtracted
+// from all later ones. `cols`: A as [j][i].
+__device__ __forceinline__ void substitute(float (&col)[16], const float* cols, uint32_t j) {
+#pragma unroll
+    for (int i = 0; i < kCell; i++) col[i] = i == int(j) ? 1.0f : 0.0f;
+#pragma unroll
+    for (int l = 0; l < kCell - 1; l++) {
+        float al[16];
+        load16(al, cols + l * kScratchRow);
+#pragma unroll
+        for (int i = l + 1; i < kCell; i++) col[i] = fmaf(-al[i], col[l], col[i]);
+    }
+}
+
+// A column as a row of the three parts of a matrix kept as [j][i].
+__device__ __forceinline__ void store_parts(float (&col)[16], char* dst) {
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = cut(col[2 * i], col[2 * i + 1]);
+        *reinterpret_cast<uint4*>(dst + p * kCell * kMatRow) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(dst + p * kCell * kMatRow + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
+// Shared memory of the forward kernel. Rows live in a ring of slots (the
+// chunk in work, the one being prepared, the ones in flight), what is
+// prepared in two stages. Matrices are kept as [j][i] (i: the step that reads,
+// j: the step that wrote), so that a lane owns a column of A.
 template <class T, int DK>
 struct Forward {
     static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-    static constexpr int kSlots = sizeof(T) == 4 ? 3 : 4;
+    static constexpr int kSlots = 4;
     static constexpr int kRow = DK * 2 + 16;                   // a bf16 part's row
     static constexpr int kRawRow = DK * int(sizeof(T)) + 16;
     static constexpr int kRawV = 64 * int(sizeof(T)) + 16;
     static constexpr int kSlotK = kCell * kRawRow, kSlotV = 2 * kSlotK, kSlotS = kSlotV + kCell * kRawV;
-    static constexpr int kSlot = kSlotS + 128;                  // q, k, v rows, then 16 log-decays and 16 betas
-    static constexpr int kStageQ = 0;
-    static constexpr int kStageK = kParts == 3 ? 3 * kCell * kRow : 0;
+    static constexpr int kSlot = kSlotS + 128 + 16;             // q, k, v rows, 16 log-decays and betas, ChunkMeta
+    static constexpr int kStageK = kParts == 3 ? 3 * kCell * kRow : 0;  // after the queries' parts
     static constexpr int kStageT = 2 * kStageK;                // three parts of (I + A)^-1
     static constexpr int kStageP = kStageT + 3 * kCell * kMatRow;
-    static constexpr int kStageVec = kStageP + 3 * kCell * kMatRow;  // g_k[16], g_q[16], c[16], g_C, ChunkMeta
-    static constexpr int kStage = kStageVec + 3 * 64 + 32;
+    static constexpr int kStageVec = kStageP + 3 * kCell * kMatRow;  // g_k[16], g_q[16], c[16], g_C
+    static constexpr int kStage = kStageVec + 3 * 64 + 16;
     static constexpr int kScratch = 2 * kCell * kScratchRow * 4 + 5 * 64;
     static constexpr size_t kSmem = size_t(kSlots) * kSlot + 2 * kStage + kScratch;
 
-    char *slots, *stages, *scratch;
+    char* smem;
 
-    __device__ explicit Forward(char* smem)
-        : slots(smem), stages(smem + kSlots * kSlot), scratch(smem + kSlots * kSlot + 2 * kStage) {}
+    __device__ explicit Forward(char* base) : smem(base) {}
+    __device__ char* slot(uint32_t i) const { return smem + i % kSlots * kSlot; }
+    __device__ char* stage(uint32_t i) const { return smem + kSlots * kSlot + (i & 1) * kStage; }
+    __device__ ChunkMeta* meta(uint32_t i) const { return reinterpret_cast<ChunkMeta*>(slot(i) + kSlotS + 128); }
+    // The bf16 parts of chunk i's queries and keys.
+    __device__ const char* queries(uint32_t i) const { return kParts == 1 ? slot(i) : stage(i); }
+    __device__ const char* keys(uint32_t i) const { return kParts == 1 ? slot(i) + kSlotK : stage(i) + kStageK; }
 
-    // The bf16 parts of a chunk's keys or queries, in the slot or the stage.
-    __device__ const char* parts(uint32_t slot, uint32_t stage, bool key) const {
-        return kParts == 1 ? slots + slot * kSlot + (key ? kSlotK : 0)
-                           : stages + stage * kStage + (key ? kStageK : kStageQ);
-    }
-
-    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, uint32_t env, uint32_t head,
-                          uint32_t qh, uint32_t v0, uint32_t lane) const {
-        char* slot = slots + m.slot * kSlot;
+    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, uint32_t i, uint32_t env,
+                          uint32_t head, uint32_t qh, uint32_t v0, uint32_t lane) const {
+        char* dst = slot(i);
+        if (lane == 0) *meta(i) = m;
         if (m.n) {
-            fetch_rows<T>(c.q, vec & 1, m.t, env, qh, 0, c.key_dim, m.n, slot, kRawRow, DK, lane);
-            fetch_rows<T>(c.k, vec & 2, m.t, env, qh, 0, c.key_dim, m.n, slot + kSlotK, kRawRow, DK, lane);
-            fetch_rows<T>(c.v, vec & 4, m.t, env, head, v0, min(64u, c.value_dim - v0), m.n, slot + kSlotV, kRawV, 64,
-                          lane);
-            fetch_scalars(c, m.t, env, head, m.n, reinterpret_cast<float*>(slot + kSlotS), lane);
+            fetch_rows<T, DK, kRawRow>(c.q, vec & 1, m.t, env, qh, 0, c.key_dim, m.n, dst, lane);
+            fetch_rows<T, DK, kRawRow>(c.k, vec & 2, m.t, env, qh, 0, c.key_dim, m.n, dst + kSlotK, lane);
+            fetch_rows<T, 64, kRawV>(c.v, vec & 4, m.t, env, head, v0, min(64u, c.value_dim - v0), m.n, dst + kSlotV,
+                                     lane);
+            fetch_scalars(c, m.t, env, head, m.n, reinterpret_cast<float*>(dst + kSlotS), lane);
         }
         cp_async_commit();
     }
 
-    // One warp: a chunk's matrices and factors, from its rows.
-    __device__ void prepare(const mdn_delta& c, const ChunkMeta& m, uint32_t stage, uint32_t lane) const {
-        char* st = stages + stage * kStage;
+    // One warp: chunk i's matrices and factors, from its rows.
+    __device__ void prepare(const mdn_delta& c, uint32_t index, uint32_t lane) const {
+        const uint32_t n = meta(index)->n;
+        if (!n) return;
+        char* st = stage(index);
         float* vec = reinterpret_cast<float*>(st + kStageVec);
-        if (lane == 0) *reinterpret_cast<ChunkMeta*>(vec + 52) = m;
-        if (!m.n) return;
-        const char* slot = slots + m.slot * kSlot;
-        if constexpr (kParts == 3) {
-            cut_rows<DK, kRow>(slot, kRawRow, st + kStageQ, lane);
-            cut_rows<DK, kRow>(slot + kSlotK, kRawRow, st + kStageK, lane);
-        }
-        float* kk = reinterpret_cast<float*>(scratch);
-        float* qk = kk + kCell * kScratchRow;
-        float* a = qk + kCell * kScratchRow;  // a[16], beta[16], 1/|k|[16], 1/|q|[16]
-        float rk = 1.0f, rq = 1.0f;
-        if (c.flags & MDN_DELTA_NORMALIZE) {
-            rq = 1.0f / sqrtf(row_squares<T, DK>(slot, kRawRow, lane) + c.norm_eps);
-            rk = 1.0f / sqrtf(row_squares<T, DK>(slot + kSlotK, kRawRow, lane) + c.norm_eps);
-        }
-        const float x = reinterpret_cast<const float*>(slot + kSlotS)[lane];
+        const char* rows = slot(index);
+        float* kk = reinterpret_cast<float*>(smem + kSlots * kSlot + 2 * kStage);
+        float* kq = kk + kCell * kScratchRow;
+        float* a = kq + kCell * kScratchRow;  // decay[16], beta[16], 1/|k|[16], scale/|q|[16], |q|^2[16]
+        const float x = reinterpret_cast<const float*>(rows + kSlotS)[lane];
         a[lane] = lane < kCell ? expf(x) : x;
-        if (!(lane & 1)) a[32 + (lane >> 1)] = rk, a[48 + (lane >> 1)] = rq;
-        __syncwarp();
-        const char *qp = parts(m.slot, stage, false), *kp = parts(m.slot, stage, true);
-        float dk0[4] = {}, dk1[4] = {}, dq0[4] = {}, dq1[4] = {};
-#pragma unroll
-        for (int kb = 0; kb < DK / 16; kb++) {
-            uint32_t ak[kParts][4], aq[kParts][4], b[kParts][4];
-#pragma unroll
-            for (int p = 0; p < kParts; p++) {
-                ldsm4(b[p], smem_addr(kp) + p * kCell * kRow + kb * 32 + lane_cols_first(lane, kRow));
-                ldsm4(ak[p], smem_addr(kp) + p * kCell * kRow + kb * 32 + lane_rows_first(lane, kRow));
-                ldsm4(aq[p], smem_addr(qp) + p * kCell * kRow + kb * 32 + lane_rows_first(lane, kRow));
-            }
-            mma_parts<kParts, kParts>(dk0, dk1, ak, b);
-            mma_parts<kParts, kParts>(dq0, dq1, aq, b);
+        if constexpr (kParts == 3) {
+            cut_rows<DK, kRow>(rows, kRawRow, st, lane);
+            cut_rows<DK, kRow>(rows + kSlotK, kRawRow, st + kStageK, lane);
+            const float squares = row_squares<DK>(rows, kRawRow, lane);
+            if (!(lane & 1)) a[64 + (lane >> 1)] = squares;
+            __syncwarp();
         }
-        const uint32_t g = lane >> 2, t = lane & 3;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float* d = kk + (g + 8 * h) * kScratchRow + 2 * t;
-            d[0] = dk0[2 * h], d[1] = dk0[2 * h + 1], d[8] = dk1[2 * h], d[9] = dk1[2 * h + 1];
-            d += kCell * kScratchRow;
-            d[0] = dq0[2 * h], d[1] = dq0[2 * h + 1], d[8] = dq1[2 * h], d[9] = dq1[2 * h + 1];
-        }
+        key_products<kParts, DK, kRow>(keys(index), queries(index), kk, kq, a + 64, lane);
         __syncwarp();
-        // Lanes 0..15 scale column j of A, lanes 16..31 that of P; decay products down the column.
+        // Lanes 0..15: step j's column of A; lanes 16..31: of P.
         const uint32_t j = lane & 15;
         const bool low = lane < 16;
-        const float bj = a[16 + j], rkj = a[32 + j];
+        float r = 1.0f;
+        if (c.flags & MDN_DELTA_NORMALIZE) r = unit_factor((low ? kk[j * (kScratchRow + 1)] : a[64 + j]) + c.norm_eps);
+        a[32 + lane] = low ? r : c.scale * r;
+        __syncwarp();
+        float col[16], decay[16], other[16];
+        load16(col, (low ? kk : kq) + j * kScratchRow);
+        load16(decay, a);
+        load16(other, a + (low ? 32 : 48));
+        const float bk = a[16 + j] * a[32 + j];
         float run = 0.0f, lead = 1.0f, tail = 0.0f;  // G_ij, g_j, G_Cj
-        float col[16];
 #pragma unroll
         for (int i = 0; i < kCell; i++) {
-            const float ai = a[i];
-            run = i == int(j) ? 1.0f : run * ai;
-            if (i <= int(j)) lead *= ai;
-            if (i + 1 == int(m.n)) tail = run;
-            const float other = low ? a[32 + i] : c.scale * a[48 + i];
-            const bool in = i < int(m.n) && (low ? i > int(j) : i >= int(j));
-            const float y = (low ? kk : qk)[i * kScratchRow + j];
-            col[i] = in ? run * other * rkj * bj * y : 0.0f;
+            run = i == int(j) ? 1.0f : run * decay[i];
+            if (i <= int(j)) lead *= decay[i];
+            if (i + 1 == int(n)) tail = run;
+            const bool in = i < int(n) && (low ? i > int(j) : i >= int(j));
+            col[i] = in ? run * other[i] * bk * col[i] : 0.0f;
         }
-        if (lane < kCell) {
-            const bool in = j < m.n;
-            vec[j] = in ? lead * rkj : 0.0f;
-            vec[16 + j] = in ? c.scale * lead * a[48 + j] : 0.0f;
-            vec[32 + j] = in ? tail * rkj * bj : 0.0f;
-            if (j + 1 == m.n) vec[48] = lead;
+        const bool in = j < n;
+        if (low) {
+            vec[j] = in ? lead * r : 0.0f;
+            vec[32 + j] = in ? tail * bk : 0.0f;
+            if (j + 1 == n) vec[48] = lead;
+        } else {
+            vec[16 + j] = in ? lead * (c.scale * r) : 0.0f;
         }
         __syncwarp();
         if (low) {
 #pragma unroll
-            for (int i = 0; i < kCell; i++) kk[i * kScratchRow + j] = col[i];
+            for (int i = 0; i < kCell; i += 4)
+                *reinterpret_cast<float4*>(kk + j * kScratchRow + i) = make_float4(col[i], col[i + 1], col[i + 2], col[i + 3]);
         }
         __syncwarp();
-        if (low) {  // column j of (I + A)^-1 by forward substitution
-#pragma unroll
-            for (int i = 0; i < kCell; i++) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int l = 0; l < i; l++) sum = fmaf(kk[i * kScratchRow + l], col[l], sum);
-                col[i] = i == int(j) ? 1.0f : -sum;
-            }
-        }
-        char* dst = st + (low ? kStageT : kStageP) + j * 2;
-#pragma unroll
-        for (int i = 0; i < kCell; i += 2) {
-            float y0 = col[i], y1 = col[i + 1];
-#pragma unroll
-            for (int p = 0; p < 3; p++) {
-                const uint32_t w = cut(y0, y1);
-                char* d = dst + p * kCell * kMatRow + i * kMatRow;
-                *reinterpret_cast<uint16_t*>(d) = uint16_t(w);
-                *reinterpret_cast<uint16_t*>(d + kMatRow) = uint16_t(w >> 16);
-            }
-        }
+        if (low) substitute(col, kk, j);
+        store_parts(col, st + (low ? kStageT : kStageP) + j * kMatRow);
     }
 };
 
@@ -576,46 +632,41 @@ __device__ __forceinline__ void store_pairs(const mdn_rows& out, bool pairs, uin
         }
 }
 
-// One CTA: 64 value columns of one environment and head; a warp for each 16 of
-// them and one warp that fetches the next chunks and prepares their matrices.
+// One CTA: 64 value columns of one environment and head. A warp for each 16 of
+// them works on chunk i while one warp prepares the matrices of chunk i + 1
+// and one fetches the rows of the chunks after it.
 template <class T, int DK>
-__global__ void __launch_bounds__(160) k_delta_rollout(const __grid_constant__ mdn_delta c, uint32_t vec) {
+__global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_constant__ mdn_delta c, uint32_t vec) {
     using F = Forward<T, DK>;
     constexpr int NP = F::kParts, NT = DK / 8;
     extern __shared__ __align__(16) char smem_raw[];
     const F f(smem_raw);
-    const uint32_t warps = blockDim.x / 32 - 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warps = blockDim.x / 32 - 2, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t env = blockIdx.x / c.heads, head = blockIdx.x % c.heads, qh = head / (c.heads / c.qk_heads);
     const uint32_t v0 = blockIdx.y * 64, live = live_steps(c, env);
-    if (warp == warps) {
+    if (warp == warps + 1) {
         ChunkWalk walk;
         walk.begin(c, env, live, lane);
-        ChunkMeta ring[F::kSlots];
-#pragma unroll
-        for (int i = 0; i < F::kSlots - 1; i++) {
-            ring[i] = walk.next(lane);
-            ring[i].slot = i;
-            f.fetch(c, vec, ring[i], env, head, qh, v0, lane);
-        }
-        cp_async_wait<F::kSlots - 2>();
-        __syncwarp();
-        f.prepare(c, ring[0], 0, lane);
+        for (uint32_t i = 0; i < F::kSlots - 1; i++) f.fetch(c, vec, walk.next(lane), i, env, head, qh, v0, lane);
+        cp_async_wait<F::kSlots - 3>();
         __syncthreads();
-        uint32_t slot = F::kSlots - 1;
-        for (uint32_t i = 0; ring[0].n; i++) {
-            ChunkMeta m = walk.next(lane);
-            m.slot = slot;
-            slot = slot + 1 == F::kSlots ? 0 : slot + 1;
-            f.fetch(c, vec, m, env, head, qh, v0, lane);
-            cp_async_wait<F::kSlots - 2>();
-            __syncwarp();
-            f.prepare(c, ring[1], (i + 1) & 1, lane);
-#pragma unroll
-            for (int r = 0; r < F::kSlots - 2; r++) ring[r] = ring[r + 1];
-            ring[F::kSlots - 2] = m;
+        __syncthreads();
+        for (uint32_t i = 0; f.meta(i)->n; i++) {
+            f.fetch(c, vec, walk.next(lane), i + F::kSlots - 1, env, head, qh, v0, lane);
+            cp_async_wait<F::kSlots - 3>();
             __syncthreads();
         }
         cp_async_wait<0>();
+        return;
+    }
+    if (warp == warps) {
+        __syncthreads();
+        f.prepare(c, 0, lane);
+        __syncthreads();
+        for (uint32_t i = 0; f.meta(i)->n; i++) {
+            f.prepare(c, i + 1, lane);
+            __syncthreads();
+        }
         return;
     }
     const uint32_t g = lane >> 2, t4 = lane & 3, col0 = v0 + warp * 16, dv = c.value_dim;
@@ -632,11 +683,11 @@ __global__ void __launch_bounds__(160) k_delta_rollout(const __grid_constant__ m
     const bool pairs = vec & 8;
     const uint32_t tiles = (dv + 15) / 16;
     __syncthreads();
+    __syncthreads();
     for (uint32_t i = 0;; i++) {
-        const uint32_t stage = i & 1;
-        const char* st = f.stages + stage * F::kStage;
+        const char* st = f.stage(i);
         const float* fac = reinterpret_cast<const float*>(st + F::kStageVec);
-        const ChunkMeta m = *reinterpret_cast<const ChunkMeta*>(fac + 52);
+        const ChunkMeta m = *f.meta(i);
         if (!m.n) break;
         if (m.fresh) {
 #pragma unroll
@@ -645,15 +696,20 @@ __global__ void __launch_bounds__(160) k_delta_rollout(const __grid_constant__ m
                 for (int e = 0; e < 4; e++) S[j][e] = 0.0f;
         }
         if (c.saved && m.t % kCell == 0 && col0 < dv) {
-            float4* d = static_cast<float4*>(c.saved) +
-                        (((size_t(m.t / kCell) * c.envs * c.heads + blockIdx.x) * tiles + col0 / 16) * NT) * 32 + lane;
+            float* d = static_cast<float*>(c.saved) +
+                       (size_t(m.t / kCell) * c.envs * c.heads + blockIdx.x) * c.key_dim * tiles * 16;
 #pragma unroll
-            for (int j = 0; j < NT; j++) d[j * 32] = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t r = 8 * j + 2 * t4 + (e & 1), col = col0 + g + 8 * (e >> 1);
+                    if (r < c.key_dim) d[size_t(r) * tiles * 16 + col] = S[j][e];
+                }
         }
-        const char* slot = f.slots + m.slot * F::kSlot;
-        const uint32_t kp = smem_addr(f.parts(m.slot, stage, true)), qp = smem_addr(f.parts(m.slot, stage, false));
+        const char* slot = f.slot(i);
+        const uint32_t kp = smem_addr(f.keys(i)), qp = smem_addr(f.queries(i));
         // S^T K^T and S^T Q^T: [16 value columns x 16 steps] each
-        float xk[2][4] = {}, xq[2][4] = {};
+        float xk[2][4] = {}, xq[2][4] = {}, ek[2][4] = {}, eq[2][4] = {};
 #pragma unroll
         for (int kb = 0; kb < DK / 16; kb++) {
             uint32_t a[3][4], bk[NP][4], bq[NP][4];
@@ -663,9 +719,13 @@ __global__ void __launch_bounds__(160) k_delta_rollout(const __grid_constant__ m
                 ldsm4(bq[p], qp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
             }
             cut_tiles<3>(S[2 * kb], S[2 * kb + 1], a);
-            mma_parts<3, NP>(xk[0], xk[1], a, bk);
-            mma_parts<3, NP>(xq[0], xq[1], a, bq);
+            mma_parts<3, NP>(xk[0], xk[1], ek[0], ek[1], a, bk);
+            mma_parts<3, NP>(xq[0], xq[1], eq[0], eq[1], a, bq);
         }
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) xk[n][e] += ek[n][e], xq[n][e] += eq[n][e];
         // X = V - g K S
         if constexpr (sizeof(T) == 2) {
             uint32_t v[4];
@@ -695,7 +755,7 @@ __global__ void __launch_bounds__(160) k_delta_rollout(const __grid_constant__ m
         cut_tiles<3>(xk[0], xk[1], parts);
 #pragma unroll
         for (int p = 0; p < 3; p++)
-            ldsm4(b[p], smem_addr(st + F::kStageT) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
+            ldsm4t(b[p], smem_addr(st + F::kStageT) + p * kCell * kMatRow + lane_rows_first(lane, kMatRow));
         mma_parts<3, 3>(w[0], w[1], parts, b);
         // S' = g_C S + (c W)^T K
         float u0[4], u1[4];
@@ -729,7 +789,7 @@ __global__ void __launch_bounds__(160) k_delta_rollout(const __grid_constant__ m
         cut_tiles<3>(w[0], w[1], parts);
 #pragma unroll
         for (int p = 0; p < 3; p++)
-            ldsm4(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
+            ldsm4t(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_rows_first(lane, kMatRow));
         mma_parts<3, 3>(xq[0], xq[1], parts, b);
 #pragma unroll
         for (int n = 0; n < 2; n++)
@@ -749,150 +809,829 @@ __global__ void __launch_bounds__(160) k_delta_rollout(const __grid_constant__ m
     }
 }
 
-// Steps back through the rollout; the state before each step is replayed from
-// the saved state of its cell.
-template <class T>
-__global__ void __launch_bounds__(kThreads) k_delta_backward(const __grid_constant__ mdn_delta c,
-                                                             const __grid_constant__ mdn_delta_grads g) {
-    extern __shared__ float smem[];
-    const uint32_t dk = c.key_dim, dv = c.value_dim;
-    float* S = smem;
-    float* dS = S + dk * dv;
-    float* q = dS + dk * dv;
-    float* k = q + dk;
-    float* u = k + dk;
-    float* dx = u + dv;
-    float* dout = dx + dv;
-    float* scratch = dout + dv;
-    const uint32_t env = blockIdx.x / c.heads, head = blockIdx.x % c.heads, group = c.heads / c.qk_heads;
-    const uint32_t qh = head / group, j = threadIdx.x, live = live_steps(c, env);
-    const size_t state = size_t(blockIdx.x) * dk * dv;
-    const float* saved = static_cast<const float*>(c.saved);
-    float* part = static_cast<float*>(g.workspace);  // [2][steps][envs][heads][dk] when heads are shared
-    const size_t part_k = size_t(c.steps) * c.envs * c.heads * dk;
-    for (uint32_t i = j; i < dk * dv; i += kThreads) dS[i] = g.dstate_out ? g.dstate_out[state + i] : 0.0f;
-    auto put = [&](uint32_t t, float dq_j, float dk_j) {
-        if (j >= dk) return;
-        if (group > 1) {
-            const size_t at = ((size_t(t) * c.envs + env) * c.heads + head) * dk + j;
-            part[at] = dq_j;
-            part[part_k + at] = dk_j;
-        } else {
-            store(row_ptr<T>(g.dq, t, env, qh) + j, dq_j);
-            store(row_ptr<T>(g.dk, t, env, qh) + j, dk_j);
-        }
-    };
-    for (uint32_t t = c.steps; t-- > live;) {
-        if (j < dv) store(row_ptr<T>(g.dv, t, env, head) + j, 0.0f);
-        put(t, 0.0f, 0.0f);
-        if (j == 0) *row_ptr<float>(g.dlog_decay, t, env, head) = 0.0f, *row_ptr<float>(g.dbeta, t, env, head) = 0.0f;
-    }
-    for (uint32_t t = live; t-- > 0;) {
-        const uint32_t cell = t / kCell;
-        __syncthreads();
-        for (uint32_t i = j; i < dk * dv; i += kThreads) {
-            const uint32_t r = i / dv, col = i % dv, lane = (col & 7) * 4 + ((r & 7) >> 1), e = (r & 1) + ((col >> 3) & 1) * 2;
-            S[i] = saved[((((size_t(cell) * c.envs * c.heads + blockIdx.x) * ((dv + 15) / 16) + col / 16) *
-                               (padded_key(dk) / 8) + r / 8) * 32 + lane) * 4 + e];
-        }
-        __syncthreads();
-        float a = 0.0f, b = 0.0f, rk = 0.0f, ks = 0.0f, v = 0.0f;
-        bool reset = false;
-        for (uint32_t r = cell * kCell; r <= t; r++) {
-            reset = c.starts && c.starts[int64_t(r) * c.starts_step + int64_t(env) * c.starts_env];
-            rk = load_row<T>(c, c.k, r, env, qh, k, scratch);
-            a = expf(*row_ptr<float>(c.log_decay, r, env, head));
-            b = *row_ptr<float>(c.beta, r, env, head);
-            if (j < dv) {
-                ks = 0.0f;
-                for (uint32_t i = 0; i < dk; i++) {
-                    const float s = reset ? 0.0f : a * S[i * dv + j];
-                    S[i * dv + j] = s;
-                    ks = fmaf(k[i], s, ks);
-                }
-                v = to_float(row_ptr<T>(c.v, r, env, head)[j]);
-                if (r < t)
-                    for (uint32_t i = 0; i < dk; i++) S[i * dv + j] = fmaf(k[i], b * (v - ks), S[i * dv + j]);
-            }
-            __syncthreads();
-        }
-        const float rq = load_row<T>(c, c.q, t, env, qh, q, scratch);
-        float db = 0.0f;
-        if (j < dv) {  // S holds a S_{t-1}; the step's own k u^T is added where it is needed
-            const float d = to_float(row_ptr<T>(g.dout, t, env, head)[j]);
-            float du = 0.0f;
-            for (uint32_t i = 0; i < dk; i++) {
-                dS[i * dv + j] = fmaf(c.scale * q[i], d, dS[i * dv + j]);
-                du = fmaf(dS[i * dv + j], k[i], du);
-            }
-            u[j] = b * (v - ks);
-            dx[j] = b * du;
-            dout[j] = d;
-            db = du * (v - ks);
-            store(row_ptr<T>(g.dv, t, env, head) + j, b * du);
-        }
-        db = block_sum(db, scratch);
-        float dqj = 0.0f, dkj = 0.0f, dg = 0.0f;
-        if (j < dk)
-            for (uint32_t e = 0; e < dv; e++) {
-                dqj = fmaf(fmaf(k[j], u[e], S[j * dv + e]), dout[e], dqj);
-                dkj = fmaf(dS[j * dv + e], u[e], dkj);
-                dkj = fmaf(-S[j * dv + e], dx[e], dkj);
-            }
-        dqj *= c.scale;
-        __syncthreads();
-        if (j < dv)
-            for (uint32_t i = 0; i < dk; i++) {
-                const float d = fmaf(-k[i], dx[j], dS[i * dv + j]);
-                dg = fmaf(d, S[i * dv + j], dg);
-                dS[i * dv + j] = reset ? 0.0f : a * d;
-            }
-        dg = block_sum(dg, scratch);
-        if (c.flags & MDN_DELTA_NORMALIZE) {
-            const float qd = block_sum(j < dk ? dqj * q[j] : 0.0f, scratch);
-            const float kd = block_sum(j < dk ? dkj * k[j] : 0.0f, scratch);
-            // One key value: x / sqrt(x^2 + eps) has the slope eps r^3; the difference below would cancel to noise.
-            if (dk == 1) dqj *= rq * rq * rq * c.norm_eps, dkj *= rk * rk * rk * c.norm_eps;
-            else if (j < dk) dqj = rq * (dqj - q[j] * qd), dkj = rk * (dkj - k[j] * kd);
-        }
-        put(t, dqj, dkj);
-        if (j == 0) *row_ptr<float>(g.dlog_decay, t, env, head) = dg, *row_ptr<float>(g.dbeta, t, env, head) = db;
-    }
-    __syncthreads();
-    if (g.dstate_in)
-        for (uint32_t i = j; i < dk * dv; i += kThreads) g.dstate_in[state + i] = dS[i];
+// -------------------------------------------------------------- gradients
+// A chunk's gradients from the state S it began with, the gradient D of the
+// state it ended with and do (w, dx, du: value vectors of a step):
+//   dU_j = sum_{i>=j} P_ij do_i + c_j D^T k_j,       P without b here,
+//   dUt = (I + A)^-T dU with A_ij = b_i G_ij (k_i.k_j),   dx_j = dv_j = b_j dUt_j,
+//   F_ij = s G_ij b_j (do_i.w_j)  (i >= j),    E_ij = -G_ij b_j (dx_i.w_j)  (i > j),
+//   dq_i = s g_i S do_i + sum_j F_ij k_j,
+//   dk_i = -g_i S dx_i + c_i b_i D w_i + sum_l F_li q_l + sum_j (E + E^T)_ij k_j,
+//   D' = g_C D + sum_i s g_i q_i do_i^T - sum_i g_i k_i dx_i^T,
+//   dbeta_j = w_j.dUt_j.
+// The decay's gradient needs no sum over states: scaling S before step t by
+// (1 + h) changes the loss by h dlog_decay_t, and the outputs and the last
+// state are linear in (S, v) together, so
+//   dlog_decay_t = <D, S_C> + sum_{r >= t in the chunk} (do_r.o_r - dv_r.v_r).
+// q_i.dq_i and k_i.dk_i, which a normalised row's gradient takes out, follow
+// from the same sums over value columns, in 32 bits whatever dq and dk are
+// stored in.
+//
+// Four warps. First each takes 16 value columns (its part of S^T and D^T in
+// registers), then, with D, w and dx in shared memory, 16 of every 64 key
+// columns of dq and dk. A fifth warp prepares the matrices of the next chunk,
+// a sixth fetches the one after.
+
+template <int N>
+__device__ __forceinline__ void cut_pair(float x, float y, uint32_t (&p)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; n++) p[n] = cut(x, y);
 }
 
-// dq and dk of shared heads: the sum of the group's parts, in head order.
+// A rollout's chunks from the last to the first.
+struct ChunkWalkBack {
+    const uint8_t* starts;
+    int64_t starts_step;
+    uint32_t live, cell_t, pos, mask, next_flag;
+    bool done;
+    __device__ void begin(const mdn_delta& c, uint32_t env, uint32_t live_steps_, uint32_t lane) {
+        starts = c.starts ? c.starts + int64_t(env) * c.starts_env : nullptr;
+        starts_step = c.starts_step;
+        live = live_steps_;
+        done = live == 0;
+        cell_t = done ? 0 : (live - 1) / kCell * kCell;
+        pos = live - cell_t;
+        mask = __ballot_sync(~0u, flag(cell_t, lane));
+        next_flag = cell_t ? flag(cell_t - kCell, lane) : 0u;
+    }
+    __device__ uint32_t flag(uint32_t t, uint32_t lane) const {
+        return starts && lane < kCell && t + lane < live ? starts[int64_t(t + lane) * starts_step] : 0u;
+    }
+    __device__ ChunkMeta next(uint32_t lane) {
+        if (done) return ChunkMeta{0, 0, 0, 0};
+        const uint32_t earlier = mask & ((1u << pos) - 1);
+        const uint32_t first = earlier ? 31 - __clz(earlier) : 0;
+        const ChunkMeta m{cell_t + first, pos - first, (mask >> first) & 1, 0};
+        pos = first;
+        if (pos == 0) {
+            done = cell_t == 0;
+            cell_t -= done ? 0 : kCell;
+            pos = kCell;
+            mask = __ballot_sync(~0u, next_flag);
+            next_flag = cell_t ? flag(cell_t - kCell, lane) : 0u;
+        }
+        return m;
+    }
+};
+
+template <class T, int DK>
+struct Backward {
+    static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;      // of q, k and do
+    static constexpr int kOut = sizeof(T) == 4 ? 3 : 2;        // of what only dq and dk are made of
+    // One stage and two slots where two and three do not fit in shared memory.
+    static constexpr bool kAhead = !(sizeof(T) == 4 && DK == 128);
+    static constexpr int kSlots = kAhead ? 3 : 2, kStages = kAhead ? 2 : 1;
+    static constexpr int kRow = DK * 2 + 16, kRowV = 64 * 2 + 16;
+    static constexpr int kRawRow = DK * int(sizeof(T)) + 16, kRawV = 64 * int(sizeof(T)) + 16;
+    static constexpr int kSlotK = kCell * kRawRow, kSlotV = 2 * kSlotK, kSlotO = kSlotV + kCell * kRawV;
+    static constexpr int kSlotS = kSlotO + kCell * kRawV, kSlot = kSlotS + 128 + 16;
+    static constexpr int kMat = 3 * kCell * kMatRow;            // three parts of a 16 x 16 matrix
+    static constexpr int kSquare = kCell * kScratchRow * 4;     // a 16 x 16 matrix of floats
+    static constexpr int kStageK = kParts == 3 ? 3 * kCell * kRow : 0;
+    static constexpr int kStageO = 2 * kStageK;
+    static constexpr int kStageW = kStageO + (kParts == 3 ? 3 * kCell * kRowV : 0);  // (I + A')^-1, as [j][i]
+    static constexpr int kStageU = kStageW + kMat;              // (I + A)^-1
+    static constexpr int kStageP = kStageU + kMat;
+    static constexpr int kStageF = kStageP + kMat;              // factors of F^T and E^T, k.q and k.k
+    static constexpr int kStageVec = kStageF + 4 * kSquare;
+    static constexpr int kStage = kStageVec + 8 * 64;
+    // after slots and stages
+    static constexpr int kD = kSlots * kSlot + kStages * kStage;   // parts of D: [part][value][key]
+    static constexpr int kW = kD + kOut * 64 * kRow;               // parts of w: [part][value][step]
+    static constexpr int kX = kW + 3 * 64 * kMatRow;               // parts of dx
+    static constexpr int kEF = kX + kOut * 64 * kMatRow;           // each warp's F^T and E^T
+    static constexpr int kFE = kEF + 4 * 2 * kSquare;              // parts of F^T and E + E^T
+    static constexpr int kSums = kFE + 2 * kOut * kCell * kMatRow;  // [warp][5][16], then rows' sums[16], <D, S>[4], S filled[4]
+    static constexpr int kScratch = kSums + 4 * 5 * 64 + 64 + 32;
+    static constexpr size_t kSmem = size_t(kScratch) + 2 * kSquare + 5 * 64;
+
+    char* smem;
+
+    __device__ explicit Backward(char* base) : smem(base) {}
+    __device__ char* slot(uint32_t i) const { return smem + i % kSlots * kSlot; }
+    __device__ char* stage(uint32_t i) const { return smem + kSlots * kSlot + i % kStages * kStage; }
+    __device__ ChunkMeta* meta(uint32_t i) const { return reinterpret_cast<ChunkMeta*>(slot(i) + kSlotS + 128); }
+    __device__ const char* queries(uint32_t i) const { return kParts == 1 ? slot(i) : stage(i); }
+    __device__ const char* keys(uint32_t i) const { return kParts == 1 ? slot(i) + kSlotK : stage(i) + kStageK; }
+    __device__ const char* douts(uint32_t i) const { return kParts == 1 ? slot(i) + kSlotO : stage(i) + kStageO; }
+
+    __device__ void fetch(const mdn_delta& c, const mdn_delta_grads& d, uint32_t vec, const ChunkMeta& m, uint32_t i,
+                          uint32_t env, uint32_t head, uint32_t qh, uint32_t v0, uint32_t lane) const {
+        char* dst = slot(i);
+        if (lane == 0) *meta(i) = m;
+        if (m.n) {
+            const uint32_t dv = min(64u, c.value_dim - v0);
+            fetch_rows<T, DK, kRawRow>(c.q, vec & 1, m.t, env, qh, 0, c.key_dim, m.n, dst, lane);
+            fetch_rows<T, DK, kRawRow>(c.k, vec & 2, m.t, env, qh, 0, c.key_dim, m.n, dst + kSlotK, lane);
+            fetch_rows<T, 64, kRawV>(c.v, vec & 4, m.t, env, head, v0, dv, m.n, dst + kSlotV, lane);
+            fetch_rows<T, 64, kRawV>(d.dout, vec & 16, m.t, env, head, v0, dv, m.n, dst + kSlotO, lane);
+            fetch_scalars(c, m.t, env, head, m.n, reinterpret_cast<float*>(dst + kSlotS), lane);
+        }
+        cp_async_commit();
+    }
+
+    // One warp: chunk i's matrices and factors.
+    __device__ void prepare(const mdn_delta& c, uint32_t index, uint32_t lane) const {
+        const uint32_t n = meta(index)->n;
+        if (!n) return;
+        char* st = stage(index);
+        // g_k, g_q, c_k, beta, decay, 1/|k|, 1/|q|, {g_C}: 16 each
+        float* vec = reinterpret_cast<float*>(st + kStageVec);
+        const char* rows = slot(index);
+        float* fe = reinterpret_cast<float*>(st + kStageF);  // F^T factors, E^T factors, k.q, k.k as [j][i]
+        float *kq = fe + 2 * kCell * kScratchRow, *kk = kq + kCell * kScratchRow;
+        float* cols = reinterpret_cast<float*>(smem + kScratch);
+        float* a = cols + 2 * kCell * kScratchRow;  // |q|^2[16]
+        const float x = reinterpret_cast<const float*>(rows + kSlotS)[lane];
+        vec[lane < kCell ? 64 + lane : 32 + lane] = lane < kCell ? expf(x) : x;
+        if constexpr (kParts == 3) {
+            cut_rows<DK, kRow>(rows, kRawRow, st, lane);
+            cut_rows<DK, kRow>(rows + kSlotK, kRawRow, st + kStageK, lane);
+            cut_rows<64, kRowV>(rows + kSlotO, kRawV, st + kStageO, lane);
+            const float squares = row_squares<DK>(rows, kRawRow, lane);
+            if (!(lane & 1)) a[lane >> 1] = squares;
+            __syncwarp();
+        }
+        key_products<kParts, DK, kRow>(keys(index), queries(index), kk, kq, a, lane);
+        __syncwarp();
+        const uint32_t j = lane & 15;
+        const bool low = lane < 16;
+        float r = 1.0f;
+        if (c.flags & MDN_DELTA_NORMALIZE) r = unit_factor((low ? kk[j * (kScratchRow + 1)] : a[j]) + c.norm_eps);
+        vec[80 + lane] = r;
+        __syncwarp();
+        // Lanes 0..15: column j of A' (and of F's factor); lanes 16..31: of A (and of E's factor).
+        float col[16], decay[16], rk[16], other[16];
+        load16(col, kk + j * kScratchRow);
+        load16(decay, vec + 64);
+        load16(rk, vec + 80);
+        load16(other, vec + (low ? 96 : 48));  // 1/|q| or beta
+        const float rkj = vec[80 + j], bj = vec[48 + j], own = low ? bj : 1.0f;
+        float run = 0.0f, lead = 1.0f, tail = 0.0f;
+        float fac[16];
+#pragma unroll
+        for (int i = 0; i < kCell; i++) {
+            run = i == int(j) ? 1.0f : run * decay[i];
+            if (i <= int(j)) lead *= decay[i];
+            if (i + 1 == int(n)) tail = run;
+            const bool below = i < int(n) && i > int(j);
+            const float pair = run * rk[i] * rkj;
+            col[i] = below ? pair * col[i] * (low ? own : other[i]) : 0.0f;
+            fac[i] = low ? (i < int(n) && i >= int(j) ? c.scale * run * other[i] * rkj * bj : 0.0f)
+                         : (below ? -pair * bj : 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < kCell; i += 4) {
+            float* d = (low ? fe : fe + kCell * kScratchRow) + j * kScratchRow + i;
+            *reinterpret_cast<float4*>(d) = make_float4(fac[i], fac[i + 1], fac[i + 2], fac[i + 3]);
+            d = (low ? cols : cols + kCell * kScratchRow) + j * kScratchRow + i;
+            *reinterpret_cast<float4*>(d) = make_float4(col[i], col[i + 1], col[i + 2], col[i + 3]);
+        }
+        const bool in = j < n;
+        if (low) {
+            vec[j] = in ? lead * rkj : 0.0f;
+            vec[32 + j] = in ? tail * rkj : 0.0f;
+            if (j + 1 == n) vec[112] = lead;
+        } else {
+            vec[16 + j] = in ? c.scale * lead * r : 0.0f;
+        }
+        __syncwarp();
+        substitute(col, (low ? cols : cols + kCell * kScratchRow), j);
+        store_parts(col, st + (low ? kStageW : kStageU) + j * kMatRow);
+        // P = scale G (k.q) / |q| / |k|: half a column a lane
+        run = 0.0f;
+        load16(other, vec + 96);
+        load16(col, kq + j * kScratchRow);
+#pragma unroll
+        for (int i = 0; i < kCell; i++) {
+            run = i == int(j) ? 1.0f : run * decay[i];
+            col[i] = i < int(n) && i >= int(j) ? c.scale * run * other[i] * rkj * col[i] : 0.0f;
+        }
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float y0 = low ? col[2 * i] : col[8 + 2 * i], y1 = low ? col[2 * i + 1] : col[9 + 2 * i];
+                w[i] = cut(y0, y1);
+                (low ? col[2 * i] : col[8 + 2 * i]) = y0;
+                (low ? col[2 * i + 1] : col[9 + 2 * i]) = y1;
+            }
+            *reinterpret_cast<uint4*>(st + kStageP + p * kCell * kMatRow + j * kMatRow + (low ? 0 : 16)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
+
+// The sums over the eight lanes g of 8 values each: value i ends in lane g = i.
+__device__ __forceinline__ float sum_over_rows(const float (&x)[8], uint32_t lane) {
+    float y[4], z[2];
+    const bool b4 = lane & 16, b2 = lane & 8, b1 = lane & 4;
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = (b4 ? x[4 + i] : x[i]) + __shfl_xor_sync(~0u, b4 ? x[i] : x[4 + i], 16);
+#pragma unroll
+    for (int i = 0; i < 2; i++) z[i] = (b2 ? y[2 + i] : y[i]) + __shfl_xor_sync(~0u, b2 ? y[i] : y[2 + i], 8);
+    return (b1 ? z[1] : z[0]) + __shfl_xor_sync(~0u, b1 ? z[0] : z[1], 4);
+}
+
+// Values of two value columns (col, col + 1) of one step.
 template <class T>
-__global__ void k_delta_group_sum(const __grid_constant__ mdn_delta c, const __grid_constant__ mdn_delta_grads g) {
-    const uint32_t dk = c.key_dim, group = c.heads / c.qk_heads;
+__device__ __forceinline__ void store_two(T* p, bool pair, uint32_t col, uint32_t cols, float x, float y) {
+    if (pair) {
+        if (col >= cols) return;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p + col) = make_float2(x, y);
+        else *reinterpret_cast<uint32_t*>(p + col) = round_pair(x, y);
+    } else {
+        if (col < cols) store(p + col, x);
+        if (col + 1 < cols) store(p + col + 1, y);
+    }
+}
+
+// Where a value block's share of dq, dk, dlog_decay and dbeta goes when other
+// value blocks or heads have shares too: parts are [steps][envs][heads][blocks].
+struct Shares {
+    float *dq, *dk, *dlog_decay, *dbeta;  // dlog_decay, dbeta only with several value blocks
+};
+__host__ __device__ inline uint32_t value_blocks(const mdn_delta& c) { return (c.value_dim + 63) / 64; }
+__host__ __device__ inline bool rows_shared(const mdn_delta& c) { return c.heads != c.qk_heads || value_blocks(c) > 1; }
+__host__ __device__ inline Shares shares_of(const mdn_delta& c, void* workspace) {
+    const size_t parts = size_t(c.steps) * c.envs * c.heads * value_blocks(c);
+    float* w = static_cast<float*>(workspace);
+    return Shares{w, w + parts * c.key_dim, w + 2 * parts * c.key_dim, w + 2 * parts * c.key_dim + parts};
+}
+
+template <class T, int DK>
+__global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_delta c,
+                                                   const __grid_constant__ mdn_delta_grads d, uint32_t vec) {
+    using F = Backward<T, DK>;
+    constexpr int NP = F::kParts, NO = F::kOut, NT = DK / 8, NS = DK / 64 ? DK / 64 : 1;
+    extern __shared__ __align__(16) char smem_raw[];
+    const F f(smem_raw);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t env = blockIdx.x / c.heads, head = blockIdx.x % c.heads, qh = head / (c.heads / c.qk_heads);
+    const uint32_t v0 = blockIdx.y * 64, live = live_steps(c, env), dk = c.key_dim, dv = c.value_dim;
+    if (warp == 5) {
+        ChunkWalkBack walk;
+        walk.begin(c, env, live, lane);
+        if constexpr (F::kAhead) {
+            f.fetch(c, d, vec, walk.next(lane), 0, env, head, qh, v0, lane);
+            f.fetch(c, d, vec, walk.next(lane), 1, env, head, qh, v0, lane);
+            cp_async_wait<0>();
+            __syncthreads();
+            __syncthreads();
+            for (uint32_t i = 0; f.meta(i)->n; i++) {
+                f.fetch(c, d, vec, walk.next(lane), i + 2, env, head, qh, v0, lane);
+                cp_async_wait<0>();
+                __syncthreads();
+            }
+        } else {
+            f.fetch(c, d, vec, walk.next(lane), 0, env, head, qh, v0, lane);
+            cp_async_wait<0>();
+            __syncthreads();
+            for (uint32_t i = 0; f.meta(i)->n; i++) {
+                f.fetch(c, d, vec, walk.next(lane), i + 1, env, head, qh, v0, lane);
+                __syncthreads();
+                cp_async_wait<0>();
+                __syncthreads();
+            }
+        }
+        return;
+    }
+    if (warp == 4) {
+        __syncthreads();
+        if constexpr (F::kAhead) {
+            f.prepare(c, 0, lane);
+            __syncthreads();
+            for (uint32_t i = 0; f.meta(i)->n; i++) {
+                f.prepare(c, i + 1, lane);
+                __syncthreads();
+            }
+        } else {
+            for (uint32_t i = 0; f.meta(i)->n; i++) {
+                f.prepare(c, i, lane);
+                __syncthreads();
+                __syncthreads();
+            }
+        }
+        return;
+    }
+    // Row g of a warp's tile is value column 2 g, row g + 8 is 2 g + 1: a lane
+    // then holds neighbours, and reads and writes them as pairs.
+    const uint32_t g = lane >> 2, t4 = lane & 3, colw = warp * 16 + 2 * g, col = v0 + colw;
+    const size_t state = size_t(blockIdx.x) * dk * dv;
+    const bool shared_rows = rows_shared(c), wide = value_blocks(c) > 1;
+    const Shares shares = shares_of(c, d.workspace);
+    float D[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t r = 8 * j + 2 * t4 + (e & 1), cc = col + (e >> 1);
+            D[j][e] = d.dstate_out && r < dk && cc < dv ? d.dstate_out[state + size_t(r) * dv + cc] : 0.0f;
+        }
+    for (uint32_t t = live; t < c.steps; t++) {
+        const size_t part = ((size_t(t) * c.envs + env) * c.heads + head) * value_blocks(c) + blockIdx.y;
+        if (t4 == 0) store_two(row_ptr<T>(d.dv, t, env, head), false, col, dv, 0.0f, 0.0f);
+        for (uint32_t i = threadIdx.x; i < dk; i += 128) {
+            if (shared_rows) shares.dq[part * dk + i] = shares.dk[part * dk + i] = 0.0f;
+            else store(row_ptr<T>(d.dq, t, env, qh) + i, 0.0f), store(row_ptr<T>(d.dk, t, env, qh) + i, 0.0f);
+        }
+        if (threadIdx.x == 0) {
+            *(wide ? shares.dlog_decay + part : row_ptr<float>(d.dlog_decay, t, env, head)) = 0.0f;
+            *(wide ? shares.dbeta + part : row_ptr<float>(d.dbeta, t, env, head)) = 0.0f;
+        }
+    }
+    const uint32_t dvp = (dv + 15) / 16 * 16;
+    float* sums = reinterpret_cast<float*>(f.smem + F::kSums);
+    float* row_sums = sums + 4 * 5 * 16;
+    float* frob = row_sums + 16;
+    __syncthreads();
+    if constexpr (F::kAhead) __syncthreads();
+    for (uint32_t i = 0;; i++) {
+        const ChunkMeta m = *f.meta(i);
+        if (!m.n) break;
+        // The state before the chunk: zeros after a start inside the cell.
+        const bool cell = m.t % kCell == 0;
+        const float* saved = static_cast<const float*>(c.saved) +
+                             (size_t(m.t / kCell) * c.envs * c.heads + blockIdx.x) * dk * dvp;
+        float S[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t r = 8 * j + 2 * t4 + e;
+                float2 x = make_float2(0.0f, 0.0f);
+                if (cell && r < dk && col < dvp) x = *reinterpret_cast<const float2*>(saved + size_t(r) * dvp + col);
+                S[j][e] = x.x, S[j][2 + e] = x.y;
+            }
+        if constexpr (!F::kAhead) __syncthreads();
+        const char* st = f.stage(i);
+        const char* slot = f.slot(i);
+        const float* fac = reinterpret_cast<const float*>(st + F::kStageVec);
+        const uint32_t kp = smem_addr(f.keys(i)), qp = smem_addr(f.queries(i)), op = smem_addr(f.douts(i));
+        const float gc = fac[112];
+
+        // ---- value columns
+        float ks[2][4] = {}, qs[2][4] = {}, dsk[2][4] = {}, frobenius = 0.0f;
+        uint32_t bits = 0;  // whether the state before the chunk is anything but zeros
+        {
+            float ek[2][4] = {}, eq[2][4] = {}, ed[2][4] = {};
+#pragma unroll
+            for (int kb = 0; kb < DK / 16; kb++) {
+                uint32_t a[3][4], bk[NP][4], bq[NP][4];
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    ldsm4(bk[p], kp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
+                    ldsm4(bq[p], qp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
+                }
+                cut_tiles<3>(S[2 * kb], S[2 * kb + 1], a);
+                mma_parts<3, NP>(ks[0], ks[1], ek[0], ek[1], a, bk);
+                mma_parts<3, NP>(qs[0], qs[1], eq[0], eq[1], a, bq);
+                cut_tiles<3>(D[2 * kb], D[2 * kb + 1], a);
+                mma_parts<3, NP>(dsk[0], dsk[1], ed[0], ed[1], a, bk);
+                // D's parts for the other warps
+                char* dst = f.smem + F::kD + colw * F::kRow + kb * 32 + 4 * t4;
+#pragma unroll
+                for (int p = 0; p < NO; p++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        *reinterpret_cast<uint32_t*>(dst + p * 64 * F::kRow + (r & 1) * F::kRow + (r >> 1) * 16) = a[p][r];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    frobenius = fmaf(D[2 * kb][e], S[2 * kb][e], frobenius);
+                    frobenius = fmaf(D[2 * kb + 1][e], S[2 * kb + 1][e], frobenius);
+                    bits |= (__float_as_uint(S[2 * kb][e]) | __float_as_uint(S[2 * kb + 1][e])) << 1;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) ks[n][e] += ek[n][e], qs[n][e] += eq[n][e], dsk[n][e] += ed[n][e];
+        }
+        // v and do of this lane's two columns and four steps 8 n + 2 t4 + (e & 1): element [n][2 * column + e]
+        float v[2][4], o[2][4];
+        uint32_t oa[NP][4];  // do^T as an A operand
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                uint32_t w[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t s = 8 * n + 2 * t4 + e;
+                    const uint32_t x = *reinterpret_cast<const uint32_t*>(slot + F::kSlotV + s * F::kRawV + colw * 2);
+                    w[e] = *reinterpret_cast<const uint32_t*>(slot + F::kSlotO + s * F::kRawV + colw * 2);
+                    v[n][e] = __uint_as_float(x << 16), v[n][2 + e] = __uint_as_float(x & 0xffff0000u);
+                    o[n][e] = __uint_as_float(w[e] << 16), o[n][2 + e] = __uint_as_float(w[e] & 0xffff0000u);
+                }
+                oa[0][2 * n] = __byte_perm(w[0], w[1], 0x5410);
+                oa[0][2 * n + 1] = __byte_perm(w[0], w[1], 0x7632);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t s = 8 * n + 2 * t4 + e;
+                    const float2 x = *reinterpret_cast<const float2*>(slot + F::kSlotV + s * F::kRawV + colw * 4);
+                    const float2 y = *reinterpret_cast<const float2*>(slot + F::kSlotO + s * F::kRawV + colw * 4);
+                    v[n][e] = x.x, v[n][2 + e] = x.y, o[n][e] = y.x, o[n][2 + e] = y.y;
+                }
+            cut_tiles<NP>(o[0], o[1], oa);
+        }
+        uint32_t a[3][4], b[3][4];
+        float w[2][4] = {}, du[2][4] = {}, dut[2][4] = {};
+        // w = (I + A')^-1 (v - g S^T k)
+        {
+            float x[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    ks[n][e] *= fac[8 * n + 2 * t4 + (e & 1)];
+                    x[n][e] = v[n][e] - ks[n][e];
+                }
+            cut_tiles<3>(x[0], x[1], a);
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+                ldsm4t(b[p], smem_addr(st + F::kStageW) + p * kCell * kMatRow + lane_rows_first(lane, kMatRow));
+            mma_parts<3, 3>(w[0], w[1], a, b);
+        }
+        // dU = P^T do + c D^T k, dUt = (I + A)^-T dU
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+            ldsm4(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
+        mma_parts<NP, 3>(du[0], du[1], oa, b);
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                dsk[n][e] *= fac[32 + 8 * n + 2 * t4 + (e & 1)];
+                du[n][e] += dsk[n][e];
+            }
+        cut_tiles<3>(du[0], du[1], a);
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+            ldsm4(b[p], smem_addr(st + F::kStageU) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
+        mma_parts<3, 3>(dut[0], dut[1], a, b);
+        // dx, dv; sums over value columns: dbeta, v.dv, g (S^T k).dx, c b (D^T k).w, g (S^T q).do
+        float dx[2][4];
+        {
+            float s0[8], s1[8], s2[8];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t s = 8 * n + 2 * t4 + e;
+                    const float beta = fac[48 + s], gq = fac[16 + s];
+                    dx[n][e] = beta * dut[n][e], dx[n][2 + e] = beta * dut[n][2 + e];
+                    const int at = 2 * n + e;
+                    s0[at] = fmaf(w[n][e], dut[n][e], w[n][2 + e] * dut[n][2 + e]);
+                    s0[4 + at] = fmaf(v[n][e], dx[n][e], v[n][2 + e] * dx[n][2 + e]);
+                    s1[at] = fmaf(ks[n][e], dx[n][e], ks[n][2 + e] * dx[n][2 + e]);
+                    s1[4 + at] = beta * fmaf(dsk[n][e], w[n][e], dsk[n][2 + e] * w[n][2 + e]);
+                    s2[at] = gq * fmaf(qs[n][e], o[n][e], qs[n][2 + e] * o[n][2 + e]);
+                    s2[4 + at] = 0.0f;
+                    if (s < m.n)
+                        store_two(row_ptr<T>(d.dv, m.t + s, env, head), vec & 8, col, dv, dx[n][e], dx[n][2 + e]);
+                }
+            s2[4] = gc * frobenius;
+            // lane g ends with sum g: kinds 2 apart, step (g & 3) -> 8 (g >> 1 & 1) + 2 t4 + (g & 1)
+            const float r0 = sum_over_rows(s0, lane), r1 = sum_over_rows(s1, lane);
+            float r2 = sum_over_rows(s2, lane);
+            const uint32_t s = ((g >> 1) & 1) * 8 + 2 * t4 + (g & 1), kind = g >> 2;
+            float* dst = sums + warp * 5 * 16;
+            dst[kind * 16 + s] = r0;
+            dst[(2 + kind) * 16 + s] = r1;
+            if (kind == 0) dst[4 * 16 + s] = r2;
+            r2 += __shfl_xor_sync(~0u, r2, 1);
+            r2 += __shfl_xor_sync(~0u, r2, 2);
+            const bool filled = __any_sync(~0u, bits != 0);
+            if (lane == 16) frob[warp] = r2, frob[4 + warp] = filled ? 1.0f : 0.0f;
+        }
+        // parts of w and dx for the key columns
+        {
+            uint32_t p[3][4];
+            cut_tiles<3>(w[0], w[1], p);
+            char* dst = f.smem + F::kW + colw * kMatRow + 4 * t4;
+#pragma unroll
+            for (int q = 0; q < 3; q++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    *reinterpret_cast<uint32_t*>(dst + q * 64 * kMatRow + (r & 1) * kMatRow + (r >> 1) * 16) = p[q][r];
+            dst = f.smem + F::kX + colw * kMatRow + 4 * t4;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                uint32_t q[NO];
+                cut_pair<NO>(dx[r >> 1][2 * (r & 1)], dx[r >> 1][2 * (r & 1) + 1], q);
+#pragma unroll
+                for (int n = 0; n < NO; n++)
+                    *reinterpret_cast<uint32_t*>(dst + n * 64 * kMatRow + (r & 1) * kMatRow + (r >> 1) * 16) = q[n];
+            }
+        }
+        __syncwarp();
+        // this warp's share of F^T and E^T: w_j . do_i and w_j . dx_i over its value columns
+        {
+            float f0[4] = {}, f1[4] = {}, e0[4] = {}, e1[4] = {};
+            uint32_t wa[3][4], ob[NP][4], xb[NO][4];
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+                ldsm4t(wa[p], smem_addr(f.smem + F::kW) + p * 64 * kMatRow + warp * 16 * kMatRow + lane_cols_first(lane, kMatRow));
+#pragma unroll
+            for (int p = 0; p < NP; p++)
+                ldsm4(ob[p], op + p * kCell * F::kRowV + warp * 32 + lane_cols_first(lane, F::kRowV));
+#pragma unroll
+            for (int p = 0; p < NO; p++)
+                ldsm4t(xb[p], smem_addr(f.smem + F::kX) + p * 64 * kMatRow + warp * 16 * kMatRow + lane_rows_first(lane, kMatRow));
+            mma_parts<3, NP>(f0, f1, wa, ob);
+            mma_out<3, NO>(e0, e1, wa, xb);
+            float* dst = reinterpret_cast<float*>(f.smem + F::kEF + warp * 2 * F::kSquare);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float* p = dst + (g + 8 * h) * kScratchRow + 2 * t4;
+                *reinterpret_cast<float2*>(p) = make_float2(f0[2 * h], f0[2 * h + 1]);
+                *reinterpret_cast<float2*>(p + 8) = make_float2(f1[2 * h], f1[2 * h + 1]);
+                p += kCell * kScratchRow;
+                *reinterpret_cast<float2*>(p) = make_float2(e0[2 * h], e0[2 * h + 1]);
+                *reinterpret_cast<float2*>(p + 8) = make_float2(e1[2 * h], e1[2 * h + 1]);
+            }
+        }
+        // D' = g_C D + (s g do)^T q - (g dx)^T k
+        {
+            uint32_t pa[3][4], pb[3][4];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t s = 8 * n + 2 * t4 + (e & 1);
+                    o[n][e] *= fac[16 + s];
+                    dx[n][e] *= -fac[s];
+                }
+            cut_tiles<3>(o[0], o[1], pa);
+            cut_tiles<3>(dx[0], dx[1], pb);
+#pragma unroll
+            for (int kb = 0; kb < DK / 16; kb++) {
+                float d0[4] = {}, d1[4] = {};
+                uint32_t bk[NP][4], bq[NP][4];
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    ldsm4t(bk[p], kp + p * kCell * F::kRow + kb * 32 + lane_rows_first(lane, F::kRow));
+                    ldsm4t(bq[p], qp + p * kCell * F::kRow + kb * 32 + lane_rows_first(lane, F::kRow));
+                }
+                mma_parts<3, NP>(d0, d1, pa, bq);
+                mma_parts<3, NP>(d0, d1, pb, bk);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    D[2 * kb][e] = m.fresh ? 0.0f : fmaf(gc, D[2 * kb][e], d0[e]);
+                    D[2 * kb + 1][e] = m.fresh ? 0.0f : fmaf(gc, D[2 * kb + 1][e], d1[e]);
+                }
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+
+        // ---- F and E: the warps' shares together, with their factors
+        {
+            const uint32_t j = threadIdx.x >> 3, i2 = (threadIdx.x & 7) * 2, at = j * kScratchRow + i2;
+            const float* part = reinterpret_cast<const float*>(f.smem + F::kEF);
+            const float* fe = reinterpret_cast<const float*>(st + F::kStageF);
+            constexpr int sq = kCell * kScratchRow;
+            float2 x = make_float2(0.0f, 0.0f), y = x;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float2 p = *reinterpret_cast<const float2*>(part + 2 * q * sq + at);
+                const float2 r = *reinterpret_cast<const float2*>(part + (2 * q + 1) * sq + at);
+                x.x += p.x, x.y += p.y, y.x += r.x, y.y += r.y;
+            }
+            const float2 ff = *reinterpret_cast<const float2*>(fe + at), ef = *reinterpret_cast<const float2*>(fe + sq + at);
+            const float2 kq = *reinterpret_cast<const float2*>(fe + 2 * sq + at);
+            const float2 kk = *reinterpret_cast<const float2*>(fe + 3 * sq + at);
+            // outside the triangle the factor is 0 and the sums belong to no product
+            x.x = ff.x != 0.0f ? x.x * ff.x : 0.0f, x.y = ff.y != 0.0f ? x.y * ff.y : 0.0f;
+            y.x = ef.x != 0.0f ? y.x * ef.x : 0.0f, y.y = ef.y != 0.0f ? y.y * ef.y : 0.0f;
+            float* back = reinterpret_cast<float*>(f.smem + F::kEF);
+            const float2 pf = make_float2(x.x * kq.x, x.y * kq.y), pe = make_float2(y.x * kk.x, y.y * kk.y);
+            *reinterpret_cast<float2*>(back + at) = pf;
+            *reinterpret_cast<float2*>(back + sq + at) = pe;
+            float row = (pf.x + pe.x) + (pf.y + pe.y);
+            row += __shfl_xor_sync(~0u, row, 1);
+            row += __shfl_xor_sync(~0u, row, 2);
+            row += __shfl_xor_sync(~0u, row, 4);
+            if ((threadIdx.x & 7) == 0) row_sums[j] = row;
+            uint32_t p[NO], q[NO];
+            cut_pair<NO>(x.x, x.y, p);
+            cut_pair<NO>(y.x, y.y, q);
+            char* dst = f.smem + F::kFE;
+            constexpr int es = NO * kCell * kMatRow;
+#pragma unroll
+            for (int n = 0; n < NO; n++) {
+                char* z = dst + n * kCell * kMatRow;
+                *reinterpret_cast<uint32_t*>(z + j * kMatRow + i2 * 2) = p[n];
+                // E^T above the diagonal (i > j), E below; the diagonal is 0
+                if (i2 >= j) {
+                    uint16_t* up = reinterpret_cast<uint16_t*>(z + es + j * kMatRow + i2 * 2);
+                    if (i2 > j) up[0] = uint16_t(q[n]);
+                    else up[0] = 0;
+                    up[1] = uint16_t(q[n] >> 16);
+                    if (i2 > j) *reinterpret_cast<uint16_t*>(z + es + i2 * kMatRow + j * 2) = uint16_t(q[n]);
+                    *reinterpret_cast<uint16_t*>(z + es + (i2 + 1) * kMatRow + j * 2) = uint16_t(q[n] >> 16);
+                } else if (i2 + 1 == j) {
+                    *reinterpret_cast<uint16_t*>(z + es + j * kMatRow + j * 2) = 0;
+                }
+            }
+        }
+        // ---- key columns: S do, S dx and D w over all value columns
+        float aq[NS][2][4] = {}, ax[NS][2][4] = {}, aw[NS][2][4] = {};
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const uint32_t k0 = (s * 4 + warp) * 16;
+            if (k0 >= DK) break;
+#pragma unroll
+            for (int vb = 0; vb < 4; vb++) {
+                uint32_t oa2[NP][4], xa[NO][4], wa[NO][4], sb[NO][4], db[NO][4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t key = k0 + g + 8 * (r >> 1), value = v0 + vb * 16 + 2 * t4 + 8 * (r & 1);
+                    float2 x = make_float2(0.0f, 0.0f);
+                    if (cell && key < dk && value < dvp)
+                        x = *reinterpret_cast<const float2*>(saved + size_t(key) * dvp + value);
+                    uint32_t p[NO];
+                    cut_pair<NO>(x.x, x.y, p);
+#pragma unroll
+                    for (int n = 0; n < NO; n++) sb[n][r] = p[n];
+                }
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+                    ldsm4(oa2[p], op + p * kCell * F::kRowV + vb * 32 + lane_rows_first(lane, F::kRowV));
+#pragma unroll
+                for (int p = 0; p < NO; p++) {
+                    ldsm4t(xa[p], smem_addr(f.smem + F::kX) + p * 64 * kMatRow + vb * 16 * kMatRow + lane_cols_first(lane, kMatRow));
+                    ldsm4t(wa[p], smem_addr(f.smem + F::kW) + p * 64 * kMatRow + vb * 16 * kMatRow + lane_cols_first(lane, kMatRow));
+                    ldsm4t(db[p], smem_addr(f.smem + F::kD) + p * 64 * F::kRow + vb * 16 * F::kRow + k0 * 2 + lane_rows_first(lane, F::kRow));
+                }
+                mma_out<NP, NO>(aq[s][0], aq[s][1], oa2, sb);
+                mma_out<NO, NO>(ax[s][0], ax[s][1], xa, sb);
+                mma_out<NO, NO>(aw[s][0], aw[s][1], wa, db);
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+
+        // q.dq and k.dk of step lane & 15: column sums of F (k.q) or E (k.k), rows' sums, sums over value columns
+        float qd, kd;
+        {
+            const float* p = reinterpret_cast<const float*>(f.smem + F::kEF) + (lane < 16 ? 0 : kCell * kScratchRow) + (lane & 15);
+            float x = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kCell; j++) x += p[j * kScratchRow];
+            const uint32_t s = lane & 15;
+            float t = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float* r = sums + q * 5 * 16 + s;
+                if (lane < 16) t += r[4 * 16];
+                else t += r[3 * 16], u += r[2 * 16];
+            }
+            x = lane < 16 ? x + t : x + row_sums[s] + (t - u);
+            const float y = __shfl_xor_sync(~0u, x, 16);
+            qd = lane < 16 ? x : y;
+            kd = lane < 16 ? y : x;
+        }
+        if (warp == 0) {  // dlog_decay and dbeta
+            const uint32_t s = lane & 15;
+            float db = 0.0f, vd = 0.0f, end = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float* r = sums + q * 5 * 16 + s;
+                db += r[0], vd += r[16], end += r[3 * 16];
+            }
+            for (int q = 8; q; q >>= 1) end += __shfl_xor_sync(~0u, end, q);
+            end += (frob[0] + frob[1]) + (frob[2] + frob[3]);
+            float dg = s < m.n ? qd - vd : 0.0f;
+#pragma unroll
+            for (int q = 1; q < 16; q <<= 1) {
+                const float x = __shfl_down_sync(~0u, dg, q, 16);
+                if (s + q < 16) dg += x;
+            }
+            dg += end;
+            // exactly 0 where the state before the step counts for nothing
+            const bool filled = frob[4] + frob[5] + frob[6] + frob[7] != 0.0f;
+            if (fac[64 + s] == 0.0f || (s == 0 && !filled)) dg = 0.0f;
+            if (lane < m.n) {
+                const size_t part = ((size_t(m.t + s) * c.envs + env) * c.heads + head) * value_blocks(c) + blockIdx.y;
+                *(wide ? shares.dlog_decay + part : row_ptr<float>(d.dlog_decay, m.t + s, env, head)) = dg;
+                *(wide ? shares.dbeta + part : row_ptr<float>(d.dbeta, m.t + s, env, head)) = db;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const uint32_t k0 = (s * 4 + warp) * 16;
+            if (k0 >= DK) break;
+            uint32_t kb[NP][4], qb[NP][4], fa[NO][4], ft[NO][4], ea[NO][4];
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                ldsm4t(kb[p], kp + p * kCell * F::kRow + k0 * 2 + lane_rows_first(lane, F::kRow));
+                ldsm4t(qb[p], qp + p * kCell * F::kRow + k0 * 2 + lane_rows_first(lane, F::kRow));
+            }
+#pragma unroll
+            for (int p = 0; p < NO; p++) {
+                const uint32_t fe = smem_addr(f.smem + F::kFE) + p * kCell * kMatRow;
+                ldsm4t(fa[p], fe + lane_cols_first(lane, kMatRow));
+                ldsm4(ft[p], fe + lane_rows_first(lane, kMatRow));
+                ldsm4(ea[p], fe + NO * kCell * kMatRow + lane_rows_first(lane, kMatRow));
+            }
+            float rq[2][4] = {}, rk[2][4] = {};
+            mma_out<NO, NP>(rq[0], rq[1], fa, kb);
+            mma_out<NO, NP>(rk[0], rk[1], ft, qb);
+            mma_out<NO, NP>(rk[0], rk[1], ea, kb);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t step = g + 8 * h;
+                const float gq = fac[16 + step], gk = fac[step], cb = fac[32 + step] * fac[48 + step];
+                const float fq = fac[96 + step] * fac[96 + step], fk = fac[80 + step] * fac[80 + step];
+                const float qdot = __shfl_sync(~0u, qd, step), kdot = __shfl_sync(~0u, kd, step);
+                const size_t part = ((size_t(m.t + step) * c.envs + env) * c.heads + head) * value_blocks(c) + blockIdx.y;
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const uint32_t key = k0 + 8 * n + 2 * t4;
+                    float yq[2], yk[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int at = 2 * h + e;
+                        yq[e] = fmaf(gq, aq[s][n][at], rq[n][at]);
+                        yk[e] = fmaf(-gk, ax[s][n][at], fmaf(cb, aw[s][n][at], rk[n][at]));
+                    }
+                    if (c.flags & MDN_DELTA_NORMALIZE) {
+                        const T* qr = reinterpret_cast<const T*>(slot + step * F::kRawRow) + key;
+                        const T* kr = reinterpret_cast<const T*>(slot + F::kSlotK + step * F::kRawRow) + key;
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            // One key value: x / sqrt(x^2 + eps) has the slope eps r^3; the difference would
+                            // cancel to noise.
+                            yq[e] = dk == 1 ? yq[e] * (c.norm_eps * fq) : fmaf(-fq * qdot, to_float(qr[e]), yq[e]);
+                            yk[e] = dk == 1 ? yk[e] * (c.norm_eps * fk) : fmaf(-fk * kdot, to_float(kr[e]), yk[e]);
+                        }
+                    }
+                    if (step >= m.n) continue;
+                    if (shared_rows) {
+                        store_two(shares.dq + part * dk, dk % 2 == 0, key, dk, yq[0], yq[1]);
+                        store_two(shares.dk + part * dk, dk % 2 == 0, key, dk, yk[0], yk[1]);
+                    } else {
+                        store_two(row_ptr<T>(d.dq, m.t + step, env, qh), vec & 32, key, dk, yq[0], yq[1]);
+                        store_two(row_ptr<T>(d.dk, m.t + step, env, qh), vec & 64, key, dk, yk[0], yk[1]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (d.dstate_in) {
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t r = 8 * j + 2 * t4 + (e & 1), cc = col + (e >> 1);
+                if (r < dk && cc < dv) d.dstate_in[state + size_t(r) * dv + cc] = D[j][e];
+            }
+    }
+}
+
+// dq and dk of a query/key head, dlog_decay and dbeta: the sums of the shares
+// of its value heads and their value blocks, in order.
+template <class T>
+__global__ void k_delta_join(const __grid_constant__ mdn_delta c, const __grid_constant__ mdn_delta_grads d) {
+    const uint32_t dk = c.key_dim, blocks = value_blocks(c), group = c.heads / c.qk_heads * blocks;
     const size_t rows = size_t(c.steps) * c.envs * c.qk_heads, total = rows * dk;
-    const float* part = static_cast<const float*>(g.workspace);
-    const size_t part_k = size_t(c.steps) * c.envs * c.heads * dk;
-    for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += size_t(gridDim.x) * blockDim.x) {
-        const uint32_t d = uint32_t(i % dk);
-        const size_t row = i / dk;
-        const uint32_t qh = uint32_t(row % c.qk_heads);
-        const size_t te = row / c.qk_heads;
-        const uint32_t env = uint32_t(te % c.envs), t = uint32_t(te / c.envs);
+    const Shares s = shares_of(c, d.workspace);
+    const size_t first = size_t(blockIdx.x) * blockDim.x + threadIdx.x, stride = size_t(gridDim.x) * blockDim.x;
+    for (size_t i = first; i < total; i += stride) {
+        const uint32_t e = uint32_t(i % dk);
+        const size_t row = i / dk, te = row / c.qk_heads;
+        const uint32_t qh = uint32_t(row % c.qk_heads), env = uint32_t(te % c.envs), t = uint32_t(te / c.envs);
         float sq = 0.0f, sk = 0.0f;
         for (uint32_t h = 0; h < group; h++) {
-            const size_t at = (te * c.heads + qh * group + h) * dk + d;
-            sq += part[at];
-            sk += part[part_k + at];
+            const size_t at = (row * group + h) * dk + e;
+            sq += s.dq[at];
+            sk += s.dk[at];
         }
-        store(row_ptr<T>(g.dq, t, env, qh) + d, sq);
-        store(row_ptr<T>(g.dk, t, env, qh) + d, sk);
+        store(row_ptr<T>(d.dq, t, env, qh) + e, sq);
+        store(row_ptr<T>(d.dk, t, env, qh) + e, sk);
+    }
+    if (blocks == 1) return;
+    const size_t scalars = size_t(c.steps) * c.envs * c.heads;
+    for (size_t i = first; i < scalars; i += stride) {
+        const uint32_t head = uint32_t(i % c.heads), env = uint32_t(i / c.heads % c.envs), t = uint32_t(i / c.heads / c.envs);
+        float dg = 0.0f, db = 0.0f;
+        for (uint32_t b = 0; b < blocks; b++) dg += s.dlog_decay[i * blocks + b], db += s.dbeta[i * blocks + b];
+        *row_ptr<float>(d.dlog_decay, t, env, head) = dg;
+        *row_ptr<float>(d.dbeta, t, env, head) = db;
     }
 }
 
 size_t saved_bytes(const mdn_delta& c) {
     const size_t cells = (size_t(c.steps) + kCell - 1) / kCell;
-    return cells * c.envs * c.heads * padded_key(c.key_dim) * ((c.value_dim + 15) / 16 * 16) * sizeof(float);
+    return cells * c.envs * c.heads * c.key_dim * ((c.value_dim + 15) / 16 * 16) * sizeof(float);
 }
 size_t workspace_bytes(const mdn_delta& c) {
-    return c.heads == c.qk_heads ? 0 : 2 * size_t(c.steps) * c.envs * c.heads * c.key_dim * sizeof(float);
+    if (!rows_shared(c)) return 0;
+    return size_t(c.steps) * c.envs * c.heads * value_blocks(c) * (2 * c.key_dim + 2) * sizeof(float);
 }
 
 void check_shape(const mdn_delta* c, const char* who) {
@@ -981,9 +1720,39 @@ void rollout(const mdn_delta& c, cudaStream_t s) {
     if (aligned_rows(c.v, e, 16)) vec |= 4;
     if (aligned_rows(c.out, e, 4) && c.value_dim % 2 == 0) vec |= 8;
     allow_smem<k_delta_rollout<T, DK>>(Forward<T, DK>::kSmem);
-    const uint32_t warps = (std::min(c.value_dim, 64u) + 15) / 16 + 1;
+    const uint32_t warps = (std::min(c.value_dim, 64u) + 15) / 16 + 2;
     const dim3 grid(c.envs * c.heads, (c.value_dim + 63) / 64);
     k_delta_rollout<T, DK><<<grid, warps * 32, Forward<T, DK>::kSmem, s>>>(c, vec);
+}
+
+template <class T, int DK>
+void gradients(const mdn_delta& c, const mdn_delta_grads& d, cudaStream_t s) {
+    constexpr uint32_t e = sizeof(T);
+    uint32_t vec = 0;
+    if (aligned_rows(c.q, e, 16)) vec |= 1;
+    if (aligned_rows(c.k, e, 16)) vec |= 2;
+    if (aligned_rows(c.v, e, 16)) vec |= 4;
+    if (aligned_rows(d.dv, e, 2 * e) && c.value_dim % 2 == 0) vec |= 8;
+    if (aligned_rows(d.dout, e, 16)) vec |= 16;
+    if (aligned_rows(d.dq, e, 2 * e) && c.key_dim % 2 == 0) vec |= 32;
+    if (aligned_rows(d.dk, e, 2 * e) && c.key_dim % 2 == 0) vec |= 64;
+    static_assert(Backward<T, DK>::kSmem <= 227 * 1024, "shared memory");
+    allow_smem<k_delta_gradients<T, DK>>(Backward<T, DK>::kSmem);
+    k_delta_gradients<T, DK><<<dim3(c.envs * c.heads, value_blocks(c)), 192, Backward<T, DK>::kSmem, s>>>(c, d, vec);
+}
+
+template <class T>
+void backward(const mdn_delta& c, const mdn_delta_grads& d, cudaStream_t s) {
+    switch (padded_key(c.key_dim)) {
+        case 32: gradients<T, 32>(c, d, s); break;
+        case 64: gradients<T, 64>(c, d, s); break;
+        default: gradients<T, 128>(c, d, s);
+    }
+    cuda_check(cudaGetLastError(), "mdn_delta_backward");
+    if (!c.steps || !rows_shared(c)) return;
+    const size_t total = size_t(c.steps) * c.envs * c.qk_heads * c.key_dim;
+    k_delta_join<T><<<unsigned(std::min<size_t>((total + 255) / 256, 148 * 16)), 256, 0, s>>>(c, d);
+    cuda_check(cudaGetLastError(), "mdn_delta_backward: shares");
 }
 
 template <class T>
@@ -1055,17 +1824,7 @@ extern "C" int mdn_delta_backward(const mdn_delta* call, const mdn_delta_grads* 
                     "mdn_delta_backward: workspace is not 16-byte aligned");
         }
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const size_t smem = (2 * size_t(c.key_dim) * c.value_dim + 2 * c.key_dim + 3 * c.value_dim + 32) * sizeof(float);
-        auto kernel = c.dtype == MDN_F32 ? k_delta_backward<float> : k_delta_backward<bf16>;
-        if (c.dtype == MDN_F32) allow_smem<k_delta_backward<float>>(227 * 1024);
-        else allow_smem<k_delta_backward<bf16>>(227 * 1024);
-        kernel<<<c.envs * c.heads, kThreads, smem, s>>>(c, g);
-        cuda_check(cudaGetLastError(), who);
-        if (c.heads != c.qk_heads && c.steps) {
-            auto sum = c.dtype == MDN_F32 ? k_delta_group_sum<float> : k_delta_group_sum<bf16>;
-            const size_t total = size_t(c.steps) * c.envs * c.qk_heads * c.key_dim;
-            sum<<<unsigned(std::min<size_t>((total + 255) / 256, 148 * 16)), 256, 0, s>>>(c, g);
-            cuda_check(cudaGetLastError(), "mdn_delta_backward: shared heads");
-        }
+        if (c.dtype == MDN_F32) backward<float>(c, g, s);
+        else backward<bf16>(c, g, s);
     });
 }
