@@ -17,6 +17,7 @@ import torch
 
 from .capi import ERR, MdnError, check, lib
 
+_Tensor = torch.Tensor
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _GATES = {"sigmoid": 0, "silu": 1}
 _NORMALIZE = 1
@@ -37,7 +38,7 @@ def _fail(message):
 
 
 def _tensor(x, name, shape, dtype, device):
-    if not isinstance(x, torch.Tensor) or x.device != device:
+    if not isinstance(x, _Tensor) or x.device != device:
         _fail(f"{name} must be a tensor on {device}")
     if x.dtype != dtype:
         _fail(f"{name} must be {dtype}, not {x.dtype}")
@@ -78,12 +79,19 @@ def _device(x, name):
     return x.device
 
 
+# the current stream's handle, without a Stream object around it (3 us a call)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _launch(device, fn, *args):
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+            status = fn(*args, _raw_stream(index))
     else:
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+        status = fn(*args, _raw_stream(index))
+    if status:
+        check(status)
 
 
 class DeltaSaved:
@@ -148,8 +156,8 @@ def delta_rule(q, k, v, log_decay, beta, state=None, *, starts=None, lengths=Non
     device = _check_delta_shape(q, v, 4)
     steps, envs = q.shape[:2]
     heads, dk, dv = v.shape[2], q.shape[3], v.shape[3]
-    out = torch.empty((steps, envs, heads, dv), dtype=q.dtype, device=device)
-    state_out = torch.empty((envs, heads, dk, dv), dtype=torch.float32, device=device)
+    out = q.new_empty((steps, envs, heads, dv))
+    state_out = q.new_empty((envs, heads, dk, dv), dtype=torch.float32)
     kept = None
     args = (q, k, v, log_decay, beta, state, starts, lengths, scale, normalize, norm_eps, state_out, out)
     if save:
@@ -196,7 +204,7 @@ def delta_step(q, k, v, log_decay, beta, state, *, starts=None, scale=None, norm
     if state is None:
         _fail("delta_step needs a state")
     if out is None:
-        out = torch.empty(v.shape, dtype=q.dtype, device=device)
+        out = q.new_empty(v.shape)
     if state_out is None:
         state_out = state
     envs, qk, dk = q.shape
@@ -280,8 +288,8 @@ def block_norm(x, branch=None, gate=None, branch_weight=None, residual_scale=Non
         _fail("y has the type of the branch, float32 or bfloat16")
     if branch is None and not next_norm:
         _fail("without a branch there is only y to compute")
-    h = x if branch is None else torch.empty(shape, dtype=x.dtype, device=device)
-    y = torch.empty(shape, dtype=kind, device=device) if next_norm else None
+    h = x if branch is None else x.new_empty(shape)
+    y = x.new_empty(shape, dtype=kind) if next_norm else None
     _launch(device, lib().mdn_block_norm_forward,
             _pack_norm(x, branch, gate, branch_weight, residual_scale, norm_weight, h if branch is not None else None, y,
                        gate_act, eps, kind, device))
