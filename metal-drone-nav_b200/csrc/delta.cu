@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) k_delta_tick(const __grid
 
 constexpr int kMatRow = 48;     // bytes of a 16-value bf16 row of a 16 x 16 matrix: 8 rows, 8 bank groups
 constexpr int kScratchRow = 20;  // floats of a 16-value row in the producer's scratch
+constexpr int kFactorRow = 36;   // the same with room for what lies past the triangle
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -200,7 +201,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -229,12 +230,13 @@ __device__ __forceinline__ void cut_tiles(const float (&t0)[4], const float (&t1
 #pragma unroll
         for (int r = 0; r < 4; r++) p[n][r] = cut(x[2 * r], x[2 * r + 1]);
 }
-// d0, d1 += A B over one k step of 16, smallest parts first.
+// d0, d1 += A B over one k step of 16, for the products of orders `from` down
+// to `to`, smallest first.
 template <int NA, int NB>
-__device__ __forceinline__ void mma_parts(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
-                                          const uint32_t (&b)[NB][4]) {
+__device__ __forceinline__ void mma_orders(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
+                                           const uint32_t (&b)[NB][4], int from, int to) {
 #pragma unroll
-    for (int order = 2; order >= 0; order--)
+    for (int order = from; order >= to; order--)
 #pragma unroll
         for (int i = 0; i < NA; i++) {
             const int j = order - i;
@@ -243,24 +245,19 @@ __device__ __forceinline__ void mma_parts(float (&d0)[4], float (&d1)[4], const 
             mma(d1, a[i], b[j][2], b[j][3]);
         }
 }
-
+template <int NA, int NB>
+__device__ __forceinline__ void mma_parts(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
+                                          const uint32_t (&b)[NB][4]) {
+    mma_orders(d0, d1, a, b, 2, 0);
+}
 // The same with the small products (order 1 and 2) in accumulators of their
 // own: the tensor cores round every accumulation toward zero, which over
 // several k steps costs bits where large and small products share a sum.
 template <int NA, int NB>
 __device__ __forceinline__ void mma_parts(float (&d0)[4], float (&d1)[4], float (&e0)[4], float (&e1)[4],
                                           const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
-#pragma unroll
-    for (int order = 2; order >= 1; order--)
-#pragma unroll
-        for (int i = 0; i < NA; i++) {
-            const int j = order - i;
-            if (j < 0 || j >= NB) continue;
-            mma(e0, a[i], b[j][0], b[j][1]);
-            mma(e1, a[i], b[j][2], b[j][3]);
-        }
-    mma(d0, a[0], b[0][0], b[0][1]);
-    mma(d1, a[0], b[0][2], b[0][3]);
+    mma_orders(e0, e1, a, b, 2, 1);
+    mma_orders(d0, d1, a, b, 0, 0);
 }
 
 // For a result that is stored as bf16 the operands have two parts and the
@@ -269,16 +266,7 @@ __device__ __forceinline__ void mma_parts(float (&d0)[4], float (&d1)[4], float 
 template <int NA, int NB>
 __device__ __forceinline__ void mma_out(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
                                         const uint32_t (&b)[NB][4]) {
-    constexpr int last = NA == 3 && NB == 3 ? 2 : NA == 2 || NB == 2 ? 1 : 2;
-#pragma unroll
-    for (int order = last; order >= 0; order--)
-#pragma unroll
-        for (int i = 0; i < NA; i++) {
-            const int j = order - i;
-            if (j < 0 || j >= NB) continue;
-            mma(d0, a[i], b[j][0], b[j][1]);
-            mma(d1, a[i], b[j][2], b[j][3]);
-        }
+    mma_orders(d0, d1, a, b, NA == 2 || NB == 2 ? 1 : 2, 0);
 }
 
 // Lane offsets of the 8 x 8 blocks that ldmatrix.x4 fetches from rows of `row`
@@ -302,44 +290,71 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// A piece of work in the stream that a CTA goes through: a chunk of an item
+// (the value columns of one block of one environment and head).
 struct ChunkMeta {
-    uint32_t t, n;      // first step, steps (0: the rollout is done)
-    uint32_t fresh;     // an episode starts at t
-    uint32_t unused;
+    uint32_t t, n;   // first step, steps (0: an item without any)
+    uint32_t flags;
+    uint32_t item;
 };
+constexpr uint32_t kFresh = 1, kFirst = 2, kLast = 4, kDone = 8;  // an episode starts at t; the item's first, last chunk
 
-// Walks a rollout's chunks in order: cells of 16 steps, cut at episode starts.
-// One warp holds it; the next cell's start flags are fetched a cell ahead.
+struct Item {
+    uint32_t bh, env, head, qh, v0;  // bh: environment x heads + head
+};
+__host__ __device__ inline uint32_t value_blocks(const mdn_delta& c) { return (c.value_dim + 63) / 64; }
+__device__ __forceinline__ Item item_of(const mdn_delta& c, uint32_t item) {
+    const uint32_t blocks = value_blocks(c), bh = item / blocks, env = bh / c.heads, head = bh - env * c.heads;
+    return Item{bh, env, head, head / (c.heads / c.qk_heads), (item - bh * blocks) * 64};
+}
+
+// Walks the chunks of items first, first + stride, ... in order: cells of 16
+// steps, cut at episode starts. One warp holds it; the next cell's start flags
+// are fetched a cell ahead.
 struct ChunkWalk {
     const uint8_t* starts;
-    int64_t starts_step;
-    uint32_t live, cell_t, pos, mask, next_flag;
-    __device__ void begin(const mdn_delta& c, uint32_t env, uint32_t live_steps_, uint32_t lane) {
-        starts = c.starts ? c.starts + int64_t(env) * c.starts_env : nullptr;
-        starts_step = c.starts_step;
-        live = live_steps_;
-        cell_t = pos = 0;
-        next_flag = flag(0, lane);
-        mask = __ballot_sync(~0u, next_flag);
-        next_flag = flag(kCell, lane);
+    uint32_t item, items, stride, live, cell_t, pos, mask, next_flag;
+    bool open;  // inside an item
+    Item at;
+    __device__ void begin(uint32_t first, uint32_t items_, uint32_t stride_) {
+        item = first, items = items_, stride = stride_, open = false;
     }
-    __device__ uint32_t flag(uint32_t t, uint32_t lane) const {
-        return starts && lane < kCell && t + lane < live ? starts[int64_t(t + lane) * starts_step] : 0u;
+    __device__ uint32_t flag(const mdn_delta& c, uint32_t t, uint32_t lane) const {
+        return starts && lane < kCell && t + lane < live ? starts[int64_t(t + lane) * c.starts_step] : 0u;
     }
-    __device__ ChunkMeta next(uint32_t lane) {
-        ChunkMeta m{cell_t + pos, 0, 0, 0};
-        if (cell_t + pos >= live) return m;
-        const uint32_t later = mask & ~((2u << pos) - 1);
-        uint32_t end = later ? __ffs(later) - 1 : kCell;
-        end = min(end, live - cell_t);
-        m.n = end - pos;
-        m.fresh = (mask >> pos) & 1;
-        pos = end;
-        if (pos == kCell) {
-            pos = 0;
-            cell_t += kCell;
-            mask = __ballot_sync(~0u, next_flag);
-            next_flag = flag(cell_t + kCell, lane);
+    __device__ ChunkMeta next(const mdn_delta& c, uint32_t lane) {
+        ChunkMeta m{0, 0, 0, item};
+        if (!open) {
+            if (item >= items) return ChunkMeta{0, 0, kDone, 0};
+            at = item_of(c, item);
+            live = live_steps(c, at.env);
+            starts = c.starts ? c.starts + int64_t(at.env) * c.starts_env : nullptr;
+            cell_t = pos = 0;
+            const uint32_t now = flag(c, 0, lane);
+            next_flag = flag(c, kCell, lane);
+            mask = __ballot_sync(~0u, now);
+            open = true;
+            m.flags = kFirst;
+        }
+        m.t = cell_t + pos;
+        if (live) {
+            const uint32_t later = mask & ~((2u << pos) - 1);
+            uint32_t end = later ? __ffs(later) - 1 : kCell;
+            end = min(end, live - cell_t);
+            m.n = end - pos;
+            if ((mask >> pos) & 1) m.flags |= kFresh;
+            pos = end;
+            if (pos == kCell) {
+                pos = 0;
+                cell_t += kCell;
+                mask = __ballot_sync(~0u, next_flag);
+                next_flag = flag(c, cell_t + kCell, lane);
+            }
+        }
+        if (cell_t + pos >= live) {
+            m.flags |= kLast;
+            open = false;
+            item = items - item > stride ? item + stride : items;
         }
         return m;
     }
@@ -443,9 +458,8 @@ __device__ __forceinline__ void key_products(const char* keys, const char* queri
         mma_parts<NP, NP>(dk0, dk1, ak, bk);
         mma_parts<NP, NP>(dq0, dq1, ak, bq);
         if constexpr (NP == 1) {
-            const uint32_t aq[4] = {bq[0][0], bq[0][2], bq[0][1], bq[0][3]};
-            mma(qq0, aq, bq[0][0], bq[0][1]);
-            mma(qq1, aq, bq[0][2], bq[0][3]);
+            const uint32_t aq[1][4] = {{bq[0][0], bq[0][2], bq[0][1], bq[0][3]}};
+            mma_parts<1, 1>(qq0, qq1, aq, bq);
         }
     }
 #pragma unroll
@@ -456,9 +470,11 @@ __device__ __forceinline__ void key_products(const char* keys, const char* queri
         *reinterpret_cast<float2*>(kq + at) = make_float2(dq0[2 * h], dq0[2 * h + 1]);
         *reinterpret_cast<float2*>(kq + at + 8) = make_float2(dq1[2 * h], dq1[2 * h + 1]);
     }
-    if (NP == 1 && t == g >> 1) {
-        squares[g] = g & 1 ? qq0[1] : qq0[0];
-        squares[8 + g] = g & 1 ? qq1[3] : qq1[2];
+    if constexpr (NP == 1) {
+        if (t == g >> 1) {
+            squares[g] = g & 1 ? qq0[1] : qq0[0];
+            squares[8 + g] = g & 1 ? qq1[3] : qq1[2];
+        }
     }
 }
 
@@ -494,318 +510,374 @@ __device__ __forceinline__ void store_parts(float (&col)[16], char* dst) {
     }
 }
 
-// Shared memory of the forward kernel. Rows live in a ring of slots (the
-// chunk in work, the one being prepared, the ones in flight), what is
-// prepared in two stages. Matrices are kept as [j][i] (i: the step that reads,
-// j: the step that wrote), so that a lane owns a column of A.
+// The forward kernel's stages, each a warp's work on a chunk of its own while
+// four warps compute chunk i: one fetches chunk i + kLead and finishes the
+// matrices of chunk i + 1, one starts those of chunk i + 2. Rows live in rings
+// of slots. i is the step that reads, j the step that wrote: c (I + A)^-1 is
+// kept as [j][i], P (I + A)^-1 as [i][j].
 template <class T, int DK>
 struct Forward {
     static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-    static constexpr int kSlots = 4;
-    static constexpr int kRow = DK * 2 + 16;                   // a bf16 part's row
+    // 32-bit rows are twice as long and have parts beside them: one chunk less in flight leaves room for two blocks.
+    static constexpr int kPending = kParts == 1 ? 1 : 0, kLead = 3 + kPending, kRing = kLead + 1;
+    static constexpr int kKeyRing = kParts == 1 ? kRing : 2;    // raw queries and keys go once their parts are there
+    static constexpr int kRow = DK * 2 + 16;                    // a bf16 part's row
     static constexpr int kRawRow = DK * int(sizeof(T)) + 16;
     static constexpr int kRawV = 64 * int(sizeof(T)) + 16;
-    static constexpr int kSlotK = kCell * kRawRow, kSlotV = 2 * kSlotK, kSlotS = kSlotV + kCell * kRawV;
-    static constexpr int kSlot = kSlotS + 128 + 16;             // q, k, v rows, 16 log-decays and betas, ChunkMeta
+    static constexpr int kKeys = 2 * kCell * kRawRow;           // queries, keys
+    static constexpr int kSlotS = kCell * kRawV, kSlot = kSlotS + 128 + 16;  // values, 16 log-decays and betas, ChunkMeta
     static constexpr int kStageK = kParts == 3 ? 3 * kCell * kRow : 0;  // after the queries' parts
-    static constexpr int kStageT = 2 * kStageK;                // three parts of (I + A)^-1
+    static constexpr int kStageT = 2 * kStageK;                 // three parts of c (I + A)^-1, then of P (I + A)^-1
     static constexpr int kStageP = kStageT + 3 * kCell * kMatRow;
     static constexpr int kStageVec = kStageP + 3 * kCell * kMatRow;  // g_k[16], g_q[16], c[16], g_C
     static constexpr int kStage = kStageVec + 3 * 64 + 16;
-    static constexpr int kScratch = 2 * kCell * kScratchRow * 4 + 5 * 64;
-    static constexpr size_t kSmem = size_t(kSlots) * kSlot + 2 * kStage + kScratch;
+    // P with its columns reversed; 15 rows for what lies past it, and before the next; -A with both axes reversed; -A
+    // as [j][i]; decay[16], zeros[16], 1/|k|[16], scale/|q|[16], and 32 that are read beside them
+    static constexpr int kBack = 31 * kFactorRow, kForth = 47 * kFactorRow, kDecay = 63 * kFactorRow;
+    static constexpr int kFactors = kDecay + 96;
+    // shared memory
+    static constexpr int kSlots = kKeyRing * kKeys, kStages = kSlots + kRing * kSlot, kFactor = kStages + 3 * kStage;
+    static constexpr int kScratch = kFactor + 2 * kFactors * 4;  // k.k, k.q, |q|^2[16]
+    static constexpr size_t kSmem = size_t(kScratch) + 2 * kCell * kScratchRow * 4 + 64;
 
     char* smem;
 
     __device__ explicit Forward(char* base) : smem(base) {}
-    __device__ char* slot(uint32_t i) const { return smem + i % kSlots * kSlot; }
-    __device__ char* stage(uint32_t i) const { return smem + kSlots * kSlot + (i & 1) * kStage; }
+    __device__ char* rows(uint32_t i) const { return smem + i % kKeyRing * kKeys; }
+    __device__ char* slot(uint32_t i) const { return smem + kSlots + i % kRing * kSlot; }
+    __device__ char* stage(uint32_t i) const { return smem + kStages + i % 3 * kStage; }
+    __device__ float* factors(uint32_t i) const { return reinterpret_cast<float*>(smem + kFactor) + (i & 1) * kFactors; }
     __device__ ChunkMeta* meta(uint32_t i) const { return reinterpret_cast<ChunkMeta*>(slot(i) + kSlotS + 128); }
     // The bf16 parts of chunk i's queries and keys.
-    __device__ const char* queries(uint32_t i) const { return kParts == 1 ? slot(i) : stage(i); }
-    __device__ const char* keys(uint32_t i) const { return kParts == 1 ? slot(i) + kSlotK : stage(i) + kStageK; }
+    __device__ const char* queries(uint32_t i) const { return kParts == 1 ? rows(i) : stage(i); }
+    __device__ const char* keys(uint32_t i) const { return kParts == 1 ? rows(i) + kCell * kRawRow : stage(i) + kStageK; }
 
-    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, uint32_t i, uint32_t env,
-                          uint32_t head, uint32_t qh, uint32_t v0, uint32_t lane) const {
+    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, const Item& at, uint32_t i,
+                          uint32_t lane) const {
         char* dst = slot(i);
         if (lane == 0) *meta(i) = m;
         if (m.n) {
-            fetch_rows<T, DK, kRawRow>(c.q, vec & 1, m.t, env, qh, 0, c.key_dim, m.n, dst, lane);
-            fetch_rows<T, DK, kRawRow>(c.k, vec & 2, m.t, env, qh, 0, c.key_dim, m.n, dst + kSlotK, lane);
-            fetch_rows<T, 64, kRawV>(c.v, vec & 4, m.t, env, head, v0, min(64u, c.value_dim - v0), m.n, dst + kSlotV,
+            fetch_rows<T, DK, kRawRow>(c.q, vec & 1, m.t, at.env, at.qh, 0, c.key_dim, m.n, rows(i), lane);
+            fetch_rows<T, DK, kRawRow>(c.k, vec & 2, m.t, at.env, at.qh, 0, c.key_dim, m.n, rows(i) + kCell * kRawRow,
+                                       lane);
+            fetch_rows<T, 64, kRawV>(c.v, vec & 4, m.t, at.env, at.head, at.v0, min(64u, c.value_dim - at.v0), m.n, dst,
                                      lane);
-            fetch_scalars(c, m.t, env, head, m.n, reinterpret_cast<float*>(dst + kSlotS), lane);
+            fetch_scalars(c, m.t, at.env, at.head, m.n, reinterpret_cast<float*>(dst + kSlotS), lane);
+        }
+        if (m.flags & kFirst && c.state_in && !(m.flags & kFresh)) {  // the state, on its way to the L2 cache
+            const char* p = reinterpret_cast<const char*>(c.state_in + size_t(at.bh) * c.key_dim * c.value_dim);
+            const uint32_t bytes = c.key_dim * c.value_dim * 4;
+            for (uint32_t b = lane * 128; b < bytes; b += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
         }
         cp_async_commit();
     }
 
-    // One warp: chunk i's matrices and factors, from its rows.
-    __device__ void prepare(const mdn_delta& c, uint32_t index, uint32_t lane) const {
-        const uint32_t n = meta(index)->n;
-        if (!n) return;
-        char* st = stage(index);
-        float* vec = reinterpret_cast<float*>(st + kStageVec);
-        const char* rows = slot(index);
-        float* kk = reinterpret_cast<float*>(smem + kSlots * kSlot + 2 * kStage);
-        float* kq = kk + kCell * kScratchRow;
-        float* a = kq + kCell * kScratchRow;  // decay[16], beta[16], 1/|k|[16], scale/|q|[16], |q|^2[16]
-        const float x = reinterpret_cast<const float*>(rows + kSlotS)[lane];
-        a[lane] = lane < kCell ? expf(x) : x;
-        if constexpr (kParts == 3) {
-            cut_rows<DK, kRow>(rows, kRawRow, st, lane);
-            cut_rows<DK, kRow>(rows + kSlotK, kRawRow, st + kStageK, lane);
-            const float squares = row_squares<DK>(rows, kRawRow, lane);
-            if (!(lane & 1)) a[64 + (lane >> 1)] = squares;
-            __syncwarp();
-        }
-        key_products<kParts, DK, kRow>(keys(index), queries(index), kk, kq, a + 64, lane);
+    // Once, before the first chunk: zeros where nothing is written later.
+    __device__ void prepare_first(uint32_t lane) const {
+        float* p = factors(0);
+        for (uint32_t i = lane; i < 2 * kFactors; i += 32) p[i] = 0.0f;
         __syncwarp();
-        // Lanes 0..15: step j's column of A; lanes 16..31: of P.
+    }
+
+    // Chunk `index`'s products of keys and queries and its decays: -A, P and the factors.
+    __device__ void start(const mdn_delta& c, uint32_t index, uint32_t lane) const {
+        const uint32_t n = meta(index)->n;
+        char* st = stage(index);
+        float* kk = reinterpret_cast<float*>(smem + kScratch);
+        float *kq = kk + kCell * kScratchRow, *squares = kq + kCell * kScratchRow;
+        float *pr = factors(index), *back = pr + kBack, *forth = pr + kForth, *a = pr + kDecay;
+        float* fac = reinterpret_cast<float*>(st + kStageVec);
+        const float x = reinterpret_cast<const float*>(slot(index) + kSlotS)[lane];  // log_decay, beta
+        const float decay = expf(x), beta = __shfl_sync(~0u, x, 16 + (lane & 15));
+        if (lane < kCell) a[lane] = decay;
+        if constexpr (kParts == 3) {
+            cut_rows<DK, kRow>(rows(index) + kCell * kRawRow, kRawRow, st + kStageK, lane);
+            const float sum = row_squares<DK>(rows(index), kRawRow, lane);
+            if (!(lane & 1)) squares[lane >> 1] = sum;
+            asm volatile("bar.sync 2, 64;" ::: "memory");  // the other warp cuts the queries
+        }
+        key_products<kParts, DK, kRow>(keys(index), queries(index), kk, kq, squares, lane);
+        // g_j = prod_{l<=j} a_l in lanes j, and G_Cj = prod_{l>j} a_l (steps past the chunk's have a = 1)
         const uint32_t j = lane & 15;
         const bool low = lane < 16;
-        float r = 1.0f;
-        if (c.flags & MDN_DELTA_NORMALIZE) r = unit_factor((low ? kk[j * (kScratchRow + 1)] : a[64 + j]) + c.norm_eps);
-        a[32 + lane] = low ? r : c.scale * r;
-        __syncwarp();
-        float col[16], decay[16], other[16];
-        load16(col, (low ? kk : kq) + j * kScratchRow);
-        load16(decay, a);
-        load16(other, a + (low ? 32 : 48));
-        const float bk = a[16 + j] * a[32 + j];
-        float run = 0.0f, lead = 1.0f, tail = 0.0f;  // G_ij, g_j, G_Cj
+        float lead = __shfl_sync(~0u, decay, j), tail = __shfl_down_sync(~0u, lead, 1, 16);
+        if (j == 15) tail = 1.0f;
 #pragma unroll
-        for (int i = 0; i < kCell; i++) {
-            run = i == int(j) ? 1.0f : run * decay[i];
-            if (i <= int(j)) lead *= decay[i];
-            if (i + 1 == int(n)) tail = run;
-            const bool in = i < int(n) && (low ? i > int(j) : i >= int(j));
-            col[i] = in ? run * other[i] * bk * col[i] : 0.0f;
+        for (int o = 1; o < 16; o <<= 1) {
+            const float up = __shfl_up_sync(~0u, lead, o, 16), down = __shfl_down_sync(~0u, tail, o, 16);
+            if (j >= uint32_t(o)) lead *= up;
+            if (j + o < 16) tail *= down;
         }
+        __syncwarp();
+        float r = 1.0f;
+        if (c.flags & MDN_DELTA_NORMALIZE) r = unit_factor((low ? kk[j * (kScratchRow + 1)] : squares[j]) + c.norm_eps);
+        a[32 + lane] = low ? r : c.scale * r;
+        const float rk = __shfl_sync(~0u, r, j);
+        __syncwarp();
         const bool in = j < n;
         if (low) {
-            vec[j] = in ? lead * r : 0.0f;
-            vec[32 + j] = in ? tail * bk : 0.0f;
-            if (j + 1 == n) vec[48] = lead;
+            fac[j] = in ? lead * r : 0.0f;
+            fac[32 + j] = in ? tail * (rk * beta) : 0.0f;
+            if (j + 1 == n) fac[48] = lead;
         } else {
-            vec[16 + j] = in ? lead * (c.scale * r) : 0.0f;
+            fac[16 + j] = in ? lead * (c.scale * r) : 0.0f;
         }
-        __syncwarp();
+        // Lanes 0..15: column j of -A below the diagonal; lanes 16..31: of P. Step by step down from the diagonal
+        // with the decays' product, so that a lane's elements are its own; past the last row the product is 0.
+        {
+            const float* dec = a + j;
+            const float* left = a + (low ? 32 : 48) + j;
+            const float* dot = (low ? kk : kq) + j * (kScratchRow + 1);
+            const float bk = low ? -(rk * beta) : rk * beta;
+            float run = 1.0f, y[16];
+#pragma unroll
+            for (int d = 0; d < kCell; d++) {  // all reads before the first write
+                if (d) run *= dec[d];
+                y[d] = run * left[d] * (bk * dot[d]);
+            }
+            // No branches: what lies past the triangle goes to rows and columns that nobody reads.
+            float* out = low ? forth + j * (kFactorRow + 1) : pr + j * kFactorRow + (15 - j);
+            float* rev = low ? back + (15 - j) * kFactorRow + (15 - j) : out;
+            const int next = low ? 1 : kFactorRow, prev = low ? -kFactorRow : kFactorRow;
+#pragma unroll
+            for (int d = 0; d < kCell; d++) {
+                *out = y[d];
+                *rev = y[d];
+                out += next;
+                rev += prev;
+            }
+        }
+    }
+
+    // What is left of chunk `index`'s matrices.
+    __device__ void finish(uint32_t index, uint32_t lane) const {
+        char* st = stage(index);
+        const float *pr = factors(index), *back = pr + kBack, *forth = pr + kForth;
+        const uint32_t j = lane & 15;
+        const bool low = lane < 16;
+        // Lanes 0..15: column j of (I + A)^-1 by forward substitution. Lanes 16..31: row j of P (I + A)^-1 from its
+        // last value to its first, the same steps on the reversed matrix. Each value goes to all later ones.
+        float col[16];
         if (low) {
 #pragma unroll
-            for (int i = 0; i < kCell; i += 4)
-                *reinterpret_cast<float4*>(kk + j * kScratchRow + i) = make_float4(col[i], col[i + 1], col[i + 2], col[i + 3]);
+            for (int i = 0; i < kCell; i++) col[i] = i == int(j) ? 1.0f : 0.0f;
+        } else {
+            load16(col, pr + j * kFactorRow);
         }
-        __syncwarp();
-        if (low) substitute(col, kk, j);
+        const float* step = low ? forth : back;
+#pragma unroll
+        for (int l = 0; l < kCell - 1; l++) {
+            float row[16];
+            load16(row, step + l * kFactorRow);
+#pragma unroll
+            for (int i = l + 1; i < kCell; i++) col[i] = fmaf(row[i], col[l], col[i]);
+        }
+        if (low) {
+            float cs[16];
+            load16(cs, reinterpret_cast<const float*>(st + kStageVec) + 32);
+#pragma unroll
+            for (int i = 0; i < kCell; i++) col[i] *= cs[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCell / 2; i++) {
+                const float y = col[i];
+                col[i] = col[15 - i];
+                col[15 - i] = y;
+            }
+        }
         store_parts(col, st + (low ? kStageT : kStageP) + j * kMatRow);
     }
 };
 
-// Values of two accumulator columns (steps) and rows (value columns) to `out`
-// rows of steps t0 + 2 t, + 1. Two lanes swap so that each stores a pair.
+// Values of two value columns (col, col + 1) of one step.
 template <class T>
-__device__ __forceinline__ void store_pairs(const mdn_rows& out, bool pairs, uint32_t t0, uint32_t n, uint32_t env,
-                                            uint32_t head, uint32_t col0, uint32_t cols, const float (&d)[4],
-                                            uint32_t step, uint32_t lane) {
-    const uint32_t g = lane >> 2;
-    if constexpr (sizeof(T) == 2) {
-        if (pairs) {
-            const bool odd = g & 1;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float got = __shfl_xor_sync(~0u, odd ? d[2 * h] : d[2 * h + 1], 4);
-                const uint32_t col = col0 + 8 * h + (g & ~1u), s = step + odd;
-                const __nv_bfloat162 w = odd ? __floats2bfloat162_rn(got, d[2 * h + 1])
-                                             : __floats2bfloat162_rn(d[2 * h], got);
-                if (s < n && col < cols)
-                    *reinterpret_cast<__nv_bfloat162*>(row_ptr<T>(out, t0 + s, env, head) + col) = w;
-            }
-            return;
-        }
+__device__ __forceinline__ void store_two(T* p, bool pair, uint32_t col, uint32_t cols, float x, float y) {
+    if (pair) {
+        if (col >= cols) return;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p + col) = make_float2(x, y);
+        else *reinterpret_cast<uint32_t*>(p + col) = round_pair(x, y);
+    } else {
+        if (col < cols) store(p + col, x);
+        if (col + 1 < cols) store(p + col + 1, y);
     }
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const uint32_t col = col0 + 8 * h + g, s = step + e;
-            if (s < n && col < cols) store(row_ptr<T>(out, t0 + s, env, head) + col, d[2 * h + e]);
-        }
 }
 
-// One CTA: 64 value columns of one environment and head. A warp for each 16 of
-// them works on chunk i while one warp prepares the matrices of chunk i + 1
-// and one fetches the rows of the chunks after it.
+// A CTA takes 64 value columns of one environment and head after the other; a
+// warp for each 16 of them.
 template <class T, int DK>
-__global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_constant__ mdn_delta c, uint32_t vec) {
+__global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_constant__ mdn_delta c, uint32_t vec,
+                                                                 uint32_t items) {
     using F = Forward<T, DK>;
     constexpr int NP = F::kParts, NT = DK / 8;
     extern __shared__ __align__(16) char smem_raw[];
     const F f(smem_raw);
     const uint32_t warps = blockDim.x / 32 - 2, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t env = blockIdx.x / c.heads, head = blockIdx.x % c.heads, qh = head / (c.heads / c.qk_heads);
-    const uint32_t v0 = blockIdx.y * 64, live = live_steps(c, env);
     if (warp == warps + 1) {
         ChunkWalk walk;
-        walk.begin(c, env, live, lane);
-        for (uint32_t i = 0; i < F::kSlots - 1; i++) f.fetch(c, vec, walk.next(lane), i, env, head, qh, v0, lane);
-        cp_async_wait<F::kSlots - 3>();
-        __syncthreads();
-        __syncthreads();
-        for (uint32_t i = 0; f.meta(i)->n; i++) {
-            f.fetch(c, vec, walk.next(lane), i + F::kSlots - 1, env, head, qh, v0, lane);
-            cp_async_wait<F::kSlots - 3>();
+        walk.begin(blockIdx.x, items, gridDim.x);
+        for (int i = -F::kLead;; i++) {
+            if (i >= 0 && f.meta(i)->flags & kDone) break;
+            if constexpr (NP == 3) {
+                if (i + 2 >= 0 && f.meta(i + 2)->n) {
+                    cut_rows<DK, F::kRow>(f.rows(i + 2), F::kRawRow, f.stage(i + 2), lane);
+                    asm volatile("bar.sync 2, 64;" ::: "memory");
+                }
+            }
+            const ChunkMeta m = walk.next(c, lane);
+            f.fetch(c, vec, m, walk.at, i + F::kLead, lane);
+            if (i + 1 >= 0 && f.meta(i + 1)->n) f.finish(i + 1, lane);
+            cp_async_wait<F::kPending>();
             __syncthreads();
         }
         cp_async_wait<0>();
         return;
     }
     if (warp == warps) {
-        __syncthreads();
-        f.prepare(c, 0, lane);
-        __syncthreads();
-        for (uint32_t i = 0; f.meta(i)->n; i++) {
-            f.prepare(c, i + 1, lane);
+        f.prepare_first(lane);
+        for (int i = -F::kLead;; i++) {
+            if (i >= 0 && f.meta(i)->flags & kDone) break;
+            if (i + 2 >= 0 && f.meta(i + 2)->n) f.start(c, i + 2, lane);
             __syncthreads();
         }
         return;
     }
-    const uint32_t g = lane >> 2, t4 = lane & 3, col0 = v0 + warp * 16, dv = c.value_dim;
-    const size_t state = size_t(blockIdx.x) * c.key_dim * dv;
+    for (int i = -F::kLead; i < 0; i++) __syncthreads();
+    // Row g of a warp's tile is value column 2 g, row g + 8 is 2 g + 1: a lane
+    // then holds neighbours, and reads and writes them as pairs.
+    const uint32_t g = lane >> 2, t4 = lane & 3, colw = warp * 16 + 2 * g, dv = c.value_dim;
+    const uint32_t dvp = (dv + 15) / 16 * 16;
     float S[NT][4];
-    const bool use_in = c.state_in && !(live && c.starts && c.starts[int64_t(env) * c.starts_env]);
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t r = 8 * j + 2 * t4 + (e & 1), col = col0 + g + 8 * (e >> 1);
-            S[j][e] = use_in && r < c.key_dim && col < dv ? c.state_in[state + size_t(r) * dv + col] : 0.0f;
-        }
-    const bool pairs = vec & 8;
-    const uint32_t tiles = (dv + 15) / 16;
-    __syncthreads();
-    __syncthreads();
     for (uint32_t i = 0;; i++) {
-        const char* st = f.stage(i);
-        const float* fac = reinterpret_cast<const float*>(st + F::kStageVec);
         const ChunkMeta m = *f.meta(i);
-        if (!m.n) break;
-        if (m.fresh) {
+        if (m.flags & kDone) break;
+        const Item at = item_of(c, m.item);
+        const uint32_t col = at.v0 + colw;
+        const size_t state = size_t(at.bh) * c.key_dim * dv;
+        if (m.flags & (kFirst | kFresh)) {
+            const bool read = c.state_in && !(m.flags & kFresh);
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) S[j][e] = 0.0f;
-        }
-        if (c.saved && m.t % kCell == 0 && col0 < dv) {
-            float* d = static_cast<float*>(c.saved) +
-                       (size_t(m.t / kCell) * c.envs * c.heads + blockIdx.x) * c.key_dim * tiles * 16;
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t r = 8 * j + 2 * t4 + (e & 1), col = col0 + g + 8 * (e >> 1);
-                    if (r < c.key_dim) d[size_t(r) * tiles * 16 + col] = S[j][e];
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t r = 8 * j + 2 * t4 + e;
+                    const float* p = c.state_in + state + size_t(r) * dv + col;
+                    const bool in = read && r < c.key_dim;
+                    float2 x = make_float2(0.0f, 0.0f);
+                    if (vec & 128) {
+                        if (in && col < dv) x = *reinterpret_cast<const float2*>(p);
+                    } else {
+                        if (in && col < dv) x.x = p[0];
+                        if (in && col + 1 < dv) x.y = p[1];
+                    }
+                    S[j][e] = x.x, S[j][2 + e] = x.y;
                 }
         }
-        const char* slot = f.slot(i);
-        const uint32_t kp = smem_addr(f.keys(i)), qp = smem_addr(f.queries(i));
-        // S^T K^T and S^T Q^T: [16 value columns x 16 steps] each
-        float xk[2][4] = {}, xq[2][4] = {}, ek[2][4] = {}, eq[2][4] = {};
+        if (m.n) {
+            const char* st = f.stage(i);
+            const float* fac = reinterpret_cast<const float*>(st + F::kStageVec);
+            if (c.saved && m.t % kCell == 0 && col < dvp) {
+                float* d = static_cast<float*>(c.saved) +
+                           (size_t(m.t / kCell) * c.envs * c.heads + at.bh) * c.key_dim * dvp + col;
 #pragma unroll
-        for (int kb = 0; kb < DK / 16; kb++) {
-            uint32_t a[3][4], bk[NP][4], bq[NP][4];
+                for (int j = 0; j < NT; j++)
 #pragma unroll
-            for (int p = 0; p < NP; p++) {
-                ldsm4(bk[p], kp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
-                ldsm4(bq[p], qp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t r = 8 * j + 2 * t4 + e;
+                        if (r < c.key_dim)
+                            *reinterpret_cast<float2*>(d + size_t(r) * dvp) = make_float2(S[j][e], S[j][2 + e]);
+                    }
             }
-            cut_tiles<3>(S[2 * kb], S[2 * kb + 1], a);
-            mma_parts<3, NP>(xk[0], xk[1], ek[0], ek[1], a, bk);
-            mma_parts<3, NP>(xq[0], xq[1], eq[0], eq[1], a, bq);
-        }
+            const char* slot = f.slot(i);
+            const uint32_t kp = smem_addr(f.keys(i)), qp = smem_addr(f.queries(i));
+            // S^T K^T and S^T Q^T: [16 value columns x 16 steps] each
+            float xk[2][4] = {}, xq[2][4] = {}, ek[2][4] = {}, eq[2][4] = {};
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+            for (int kb = 0; kb < DK / 16; kb++) {
+                uint32_t a[3][4], bk[NP][4], bq[NP][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) xk[n][e] += ek[n][e], xq[n][e] += eq[n][e];
-        // X = V - g K S
-        if constexpr (sizeof(T) == 2) {
-            uint32_t v[4];
-            ldsm4t(v, smem_addr(slot + F::kSlotV + warp * 32) + lane_cols_first(lane, F::kRawV));
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const float g0 = fac[8 * n + 2 * t4], g1 = fac[8 * n + 2 * t4 + 1];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    xk[n][2 * h] = __uint_as_float(v[2 * n + h] << 16) - g0 * xk[n][2 * h];
-                    xk[n][2 * h + 1] = __uint_as_float(v[2 * n + h] & 0xffff0000u) - g1 * xk[n][2 * h + 1];
+                for (int p = 0; p < NP; p++) {
+                    ldsm4(bk[p], kp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
+                    ldsm4(bq[p], qp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
                 }
+                cut_tiles<3>(S[2 * kb], S[2 * kb + 1], a);
+                mma_parts<3, NP>(xk[0], xk[1], ek[0], ek[1], a, bk);
+                mma_parts<3, NP>(xq[0], xq[1], eq[0], eq[1], a, bq);
             }
-        } else {
+            // X = V - g K S, and g Q S
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t s = 8 * n + 2 * t4 + (e & 1);
-                    const float v = reinterpret_cast<const float*>(slot + F::kSlotV + s * F::kRawV)[warp * 16 + g + 8 * (e >> 1)];
-                    xk[n][e] = v - fac[s] * xk[n][e];
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t s = 8 * n + 2 * t4 + e;
+                    float v0, v1;
+                    if constexpr (sizeof(T) == 2) {
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(slot + s * F::kRawV + colw * 2);
+                        v0 = __uint_as_float(x << 16), v1 = __uint_as_float(x & 0xffff0000u);
+                    } else {
+                        const float2 x = *reinterpret_cast<const float2*>(slot + s * F::kRawV + colw * 4);
+                        v0 = x.x, v1 = x.y;
+                    }
+                    const float gk = fac[s], gq = fac[16 + s];
+                    xk[n][e] = fmaf(-gk, xk[n][e] + ek[n][e], v0);
+                    xk[n][2 + e] = fmaf(-gk, xk[n][2 + e] + ek[n][2 + e], v1);
+                    xq[n][e] = gq * (xq[n][e] + eq[n][e]);
+                    xq[n][2 + e] = gq * (xq[n][2 + e] + eq[n][2 + e]);
                 }
-        }
-        // W = (I + A)^-1 X
-        float w[2][4] = {};
-        uint32_t parts[3][4], b[3][4];
-        cut_tiles<3>(xk[0], xk[1], parts);
+            // c W and O = g Q S + P W, W = (I + A)^-1 X
+            float u[2][4] = {}, o[2][4] = {};
+            uint32_t parts[3][4], b[3][4];
+            cut_tiles<3>(xk[0], xk[1], parts);
 #pragma unroll
-        for (int p = 0; p < 3; p++)
-            ldsm4t(b[p], smem_addr(st + F::kStageT) + p * kCell * kMatRow + lane_rows_first(lane, kMatRow));
-        mma_parts<3, 3>(w[0], w[1], parts, b);
-        // S' = g_C S + (c W)^T K
-        float u0[4], u1[4];
+            for (int p = 0; p < 3; p++)
+                ldsm4t(b[p], smem_addr(st + F::kStageT) + p * kCell * kMatRow + lane_rows_first(lane, kMatRow));
+            mma_parts<3, 3>(u[0], u[1], parts, b);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            u0[e] = w[0][e] * fac[32 + 2 * t4 + (e & 1)];
-            u1[e] = w[1][e] * fac[40 + 2 * t4 + (e & 1)];
-        }
-        cut_tiles<3>(u0, u1, parts);
-        const float gc = fac[48];
+            for (int p = 0; p < 3; p++)
+                ldsm4(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
+            mma_parts<3, 3>(o[0], o[1], parts, b);
+            T* out = row_ptr<T>(c.out, m.t, at.env, at.head);
 #pragma unroll
-        for (int kb = 0; kb < DK / 16; kb++) {
-            float d0[4] = {}, d1[4] = {};
-            uint32_t bk[NP][4];
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int p = 0; p < NP; p++)
-                ldsm4t(bk[p], kp + p * kCell * F::kRow + kb * 32 + lane_rows_first(lane, F::kRow));
-            mma_parts<3, NP>(d0, d1, parts, bk);
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t s = 8 * n + 2 * t4 + e;
+                    if (s < m.n)
+                        store_two(out + int64_t(s) * c.out.step, vec & 8, col, dv, o[n][e] + xq[n][e],
+                                  o[n][2 + e] + xq[n][2 + e]);
+                }
+            // S' = g_C S + (c W)^T K
+            cut_tiles<3>(u[0], u[1], parts);
+            const float gc = fac[48];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                S[2 * kb][e] = fmaf(gc, S[2 * kb][e], d0[e]);
-                S[2 * kb + 1][e] = fmaf(gc, S[2 * kb + 1][e], d1[e]);
+            for (int kb = 0; kb < DK / 16; kb++) {
+                float d0[4] = {}, d1[4] = {};
+                uint32_t bk[NP][4];
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+                    ldsm4t(bk[p], kp + p * kCell * F::kRow + kb * 32 + lane_rows_first(lane, F::kRow));
+                mma_parts<3, NP>(d0, d1, parts, bk);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    S[2 * kb][e] = fmaf(gc, S[2 * kb][e], d0[e]);
+                    S[2 * kb + 1][e] = fmaf(gc, S[2 * kb + 1][e], d1[e]);
+                }
             }
         }
-        // O = g Q S + P W
+        if (m.flags & kLast) {
+            for (uint32_t t = m.t + m.n; t < c.steps; t++)
+                if (t4 == 0) store_two(row_ptr<T>(c.out, t, at.env, at.head), false, col, dv, 0.0f, 0.0f);
+            if (c.state_out) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            xq[0][e] *= fac[16 + 2 * t4 + (e & 1)];
-            xq[1][e] *= fac[24 + 2 * t4 + (e & 1)];
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t r = 8 * j + 2 * t4 + e;
+                        if (r < c.key_dim)
+                            store_two(c.state_out + state + size_t(r) * dv, vec & 128, col, dv, S[j][e], S[j][2 + e]);
+                    }
+            }
         }
-        cut_tiles<3>(w[0], w[1], parts);
-#pragma unroll
-        for (int p = 0; p < 3; p++)
-            ldsm4t(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_rows_first(lane, kMatRow));
-        mma_parts<3, 3>(xq[0], xq[1], parts, b);
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-            store_pairs<T>(c.out, pairs, m.t, m.n, env, head, col0, dv, xq[n], 8 * n + 2 * t4, lane);
         __syncthreads();
-    }
-    for (uint32_t t = live; t < c.steps; t++)
-        if (lane < 16 && col0 + lane < dv) store(row_ptr<T>(c.out, t, env, head) + col0 + lane, 0.0f);
-    if (c.state_out) {
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t r = 8 * j + 2 * t4 + (e & 1), col = col0 + g + 8 * (e >> 1);
-                if (r < c.key_dim && col < dv) c.state_out[state + size_t(r) * dv + col] = S[j][e];
-            }
     }
 }
 
@@ -858,10 +930,10 @@ struct ChunkWalkBack {
         return starts && lane < kCell && t + lane < live ? starts[int64_t(t + lane) * starts_step] : 0u;
     }
     __device__ ChunkMeta next(uint32_t lane) {
-        if (done) return ChunkMeta{0, 0, 0, 0};
+        if (done) return ChunkMeta{0, 0, kDone, 0};
         const uint32_t earlier = mask & ((1u << pos) - 1);
         const uint32_t first = earlier ? 31 - __clz(earlier) : 0;
-        const ChunkMeta m{cell_t + first, pos - first, (mask >> first) & 1, 0};
+        const ChunkMeta m{cell_t + first, pos - first, (mask >> first) & 1 ? kFresh : 0u, 0};
         pos = first;
         if (pos == 0) {
             done = cell_t == 0;
@@ -1034,25 +1106,11 @@ __device__ __forceinline__ float sum_over_rows(const float (&x)[8], uint32_t lan
     return (b1 ? z[1] : z[0]) + __shfl_xor_sync(~0u, b1 ? z[0] : z[1], 4);
 }
 
-// Values of two value columns (col, col + 1) of one step.
-template <class T>
-__device__ __forceinline__ void store_two(T* p, bool pair, uint32_t col, uint32_t cols, float x, float y) {
-    if (pair) {
-        if (col >= cols) return;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p + col) = make_float2(x, y);
-        else *reinterpret_cast<uint32_t*>(p + col) = round_pair(x, y);
-    } else {
-        if (col < cols) store(p + col, x);
-        if (col + 1 < cols) store(p + col + 1, y);
-    }
-}
-
 // Where a value block's share of dq, dk, dlog_decay and dbeta goes when other
 // value blocks or heads have shares too: parts are [steps][envs][heads][blocks].
 struct Shares {
     float *dq, *dk, *dlog_decay, *dbeta;  // dlog_decay, dbeta only with several value blocks
 };
-__host__ __device__ inline uint32_t value_blocks(const mdn_delta& c) { return (c.value_dim + 63) / 64; }
 __host__ __device__ inline bool rows_shared(const mdn_delta& c) { return c.heads != c.qk_heads || value_blocks(c) > 1; }
 __host__ __device__ inline Shares shares_of(const mdn_delta& c, void* workspace) {
     const size_t parts = size_t(c.steps) * c.envs * c.heads * value_blocks(c);
@@ -1381,8 +1439,8 @@ __global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_d
                 mma_parts<3, NP>(d0, d1, pb, bk);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    D[2 * kb][e] = m.fresh ? 0.0f : fmaf(gc, D[2 * kb][e], d0[e]);
-                    D[2 * kb + 1][e] = m.fresh ? 0.0f : fmaf(gc, D[2 * kb + 1][e], d1[e]);
+                    D[2 * kb][e] = m.flags & kFresh ? 0.0f : fmaf(gc, D[2 * kb][e], d0[e]);
+                    D[2 * kb + 1][e] = m.flags & kFresh ? 0.0f : fmaf(gc, D[2 * kb + 1][e], d1[e]);
                 }
             }
         }
@@ -1644,7 +1702,7 @@ void check_shape(const mdn_delta* c, const char* who) {
             MDN_ERR_INVALID, at + "key_dim and value_dim must be 1..128");
     require(c->dtype == MDN_F32 || c->dtype == MDN_BF16, MDN_ERR_INVALID, at + "dtype must be MDN_F32 or MDN_BF16");
     require((c->flags & ~MDN_DELTA_NORMALIZE) == 0, MDN_ERR_INVALID, at + "unknown flags");
-    require(uint64_t(c->envs) * c->heads <= 0x7fffffffu, MDN_ERR_INVALID, at + "envs x heads exceeds 2^31 - 1");
+    require(uint64_t(c->envs) * c->heads <= 0x3fffffffu, MDN_ERR_INVALID, at + "envs x heads exceeds 2^30 - 1");
     require(c->steps <= 0x7fffffffu, MDN_ERR_INVALID, at + "steps exceeds 2^31 - 1");
 }
 
@@ -1667,16 +1725,23 @@ void check_inputs(const mdn_delta* c, const char* who) {
             std::string(who) + ": saved is not 16-byte aligned");
 }
 
-// Lets a kernel use `bytes` of shared memory, once per device.
+// Lets a kernel use `bytes` of shared memory, and how many of its blocks the
+// device holds at once: asked once per device.
 template <auto Kernel>
-void allow_smem(size_t bytes) {
-    static std::atomic<uint64_t> done{0};
+uint32_t resident_blocks(size_t bytes, int threads) {
+    constexpr int kDevices = 64;
+    static std::atomic<uint32_t> known[kDevices];
     int dev = 0;
     cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if (done.load(std::memory_order_relaxed) & bit) return;
+    if (dev < kDevices)
+        if (const uint32_t blocks = known[dev].load(std::memory_order_relaxed)) return blocks;
+    int per_sm = 0, sms = 0;
     cuda_check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "shared memory");
-    done.fetch_or(bit, std::memory_order_relaxed);
+    cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, Kernel, threads, bytes), "occupancy");
+    cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "SM count");
+    const uint32_t blocks = uint32_t(std::max(1, per_sm * sms));
+    if (dev < kDevices) known[dev].store(blocks, std::memory_order_relaxed);
+    return blocks;
 }
 
 // Whether rows start on `bytes`-byte boundaries whatever the step, environment and head.
@@ -1718,11 +1783,13 @@ void rollout(const mdn_delta& c, cudaStream_t s) {
     if (aligned_rows(c.q, e, 16)) vec |= 1;
     if (aligned_rows(c.k, e, 16)) vec |= 2;
     if (aligned_rows(c.v, e, 16)) vec |= 4;
-    if (aligned_rows(c.out, e, 4) && c.value_dim % 2 == 0) vec |= 8;
-    allow_smem<k_delta_rollout<T, DK>>(Forward<T, DK>::kSmem);
-    const uint32_t warps = (std::min(c.value_dim, 64u) + 15) / 16 + 2;
-    const dim3 grid(c.envs * c.heads, (c.value_dim + 63) / 64);
-    k_delta_rollout<T, DK><<<grid, warps * 32, Forward<T, DK>::kSmem, s>>>(c, vec);
+    if (aligned_rows(c.out, e, 2 * e) && c.value_dim % 2 == 0) vec |= 8;
+    const uintptr_t states = reinterpret_cast<uintptr_t>(c.state_in) | reinterpret_cast<uintptr_t>(c.state_out);
+    if (states % 8 == 0 && c.value_dim % 2 == 0) vec |= 128;
+    static_assert(Forward<T, DK>::kSmem <= 227 * 1024, "shared memory");
+    const uint32_t threads = ((std::min(c.value_dim, 64u) + 15) / 16 + 2) * 32, items = c.envs * c.heads * value_blocks(c);
+    const uint32_t blocks = resident_blocks<k_delta_rollout<T, DK>>(Forward<T, DK>::kSmem, 192);
+    k_delta_rollout<T, DK><<<std::min(items, blocks), threads, Forward<T, DK>::kSmem, s>>>(c, vec, items);
 }
 
 template <class T, int DK>
@@ -1737,7 +1804,7 @@ void gradients(const mdn_delta& c, const mdn_delta_grads& d, cudaStream_t s) {
     if (aligned_rows(d.dq, e, 2 * e) && c.key_dim % 2 == 0) vec |= 32;
     if (aligned_rows(d.dk, e, 2 * e) && c.key_dim % 2 == 0) vec |= 64;
     static_assert(Backward<T, DK>::kSmem <= 227 * 1024, "shared memory");
-    allow_smem<k_delta_gradients<T, DK>>(Backward<T, DK>::kSmem);
+    resident_blocks<k_delta_gradients<T, DK>>(Backward<T, DK>::kSmem, 192);
     k_delta_gradients<T, DK><<<dim3(c.envs * c.heads, value_blocks(c)), 192, Backward<T, DK>::kSmem, s>>>(c, d, vec);
 }
 
