@@ -38,55 +38,70 @@ __device__ __forceinline__ uint32_t live_steps(const mdn_delta& c, uint32_t env)
     return n <= 0 ? 0u : min(uint32_t(n), c.steps);
 }
 
+// 1 / sqrt(x), the hardware's estimate with a Newton step.
+__device__ __forceinline__ float unit_factor(float x) {
+    const float r = rsqrtf(x);
+    return x > 0.0f && r > 0.0f ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
+}
+
 // ------------------------------------------------------------------ tick
 // One step (the policy tick): the state is read once, held in registers, and
 // written once. Bound by those bytes. Both products with the state are taken
 // in the one pass, with o = s (a S)^T q + s (q.k) u in place of a second pass
 // over the new state. A group of GT threads holds one state, 32 values a
-// thread: column units of V values (V = 4: 16-byte accesses) across lanes, the
-// rows dealt to the RG = GT / CP row groups. GT = 32 keeps all sums inside a
-// warp; larger states join their warps' sums in shared memory.
+// thread: column units of V values (V = 4: 16-byte accesses) across lanes, and
+// NI = 32 / V consecutive rows for each of the GT / CP row groups. GT = 32
+// keeps all sums inside a warp; larger states join their warps' sums in shared
+// memory.
 template <class T, int V, int GT>
-__global__ void __launch_bounds__(GT < 128 ? 128 : GT) k_delta_tick(const __grid_constant__ mdn_delta c, int log_cp) {
+__global__ void __launch_bounds__(GT < 128 ? 128 : GT, V == 4 && GT >= 128 ? 768 / GT : 0) k_delta_tick(const __grid_constant__ mdn_delta c, int log_cp) {
     constexpr int NI = 32 / V, kWarps = GT / 32, kGroups = GT < 128 ? 128 / GT : 1;
-    constexpr int kRow = 128;  // widest column axis
-    __shared__ float sums[kWarps > 1 ? kWarps : 1][2][kWarps > 1 ? kRow : 1];
+    constexpr int kWide = 128;  // the widest axis
+    __shared__ float sums[kWarps > 1 ? kWarps : 1][2][kWarps > 1 ? kWide : 1];
+    __shared__ __align__(16) float keys[kGroups][2][kWide];  // k, q; zeros past the last
     const uint32_t item = blockIdx.x * kGroups + threadIdx.x / GT, tid = threadIdx.x % GT, lane = threadIdx.x & 31;
     if (item >= c.envs * c.heads) return;  // only whole groups leave, and only where groups are warps
     const uint32_t env = item / c.heads, head = item % c.heads, qh = head / (c.heads / c.qk_heads);
     const uint32_t dk = c.key_dim, dv = c.value_dim;
-    const uint32_t col = (tid & ((1u << log_cp) - 1)) * V, rg = tid >> log_cp, nrg = GT >> log_cp;
+    const uint32_t col = (tid & ((1u << log_cp) - 1)) * V, r0 = (tid >> log_cp) * NI;
     const bool mine = col < dv;
     const size_t state = size_t(item) * dk * dv;
     const bool live = live_steps(c, env) != 0;
     const bool fresh = live && c.starts && c.starts[int64_t(env) * c.starts_env];
     float S[NI][V];
+    const float* p = c.state_in + state + size_t(r0) * dv + col;
+    const bool read = mine && c.state_in && !fresh;
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-        const uint32_t r = rg + i * nrg;
+    for (int i = 0; i < NI; i++, p += dv) {
 #pragma unroll
         for (int e = 0; e < V; e++) S[i][e] = 0.0f;
-        if (mine && r < dk && c.state_in && !fresh) {
-            const float* p = c.state_in + state + size_t(r) * dv + col;
+        if (read && r0 + i < dk) {
             if constexpr (V == 4) {
                 const float4 x = __ldcs(reinterpret_cast<const float4*>(p));
                 S[i][0] = x.x, S[i][1] = x.y, S[i][2] = x.z, S[i][3] = x.w;
             } else {
-                S[i][0] = *p;
+                S[i][0] = __ldcs(p);
             }
         }
     }
     if (live) {
+        float(&keyq)[2][kWide] = keys[threadIdx.x / GT];
         const T* qp = row_ptr<T>(c.q, 0, env, qh);
         const T* kp = row_ptr<T>(c.k, 0, env, qh);
+        for (uint32_t i = tid; i < kWide; i += GT) {
+            keyq[0][i] = i < dk ? to_float(kp[i]) : 0.0f;
+            keyq[1][i] = i < dk ? to_float(qp[i]) : 0.0f;
+        }
         const float a = expf(*row_ptr<float>(c.log_decay, 0, env, head));
         const float b = *row_ptr<float>(c.beta, 0, env, head);
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; e++) v[e] = mine ? to_float(row_ptr<T>(c.v, 0, env, head)[col + e]) : 0.0f;
+        if constexpr (kWarps > 1) __syncthreads();
+        else __syncwarp();
         float qq = 0.0f, kk = 0.0f, qk = 0.0f;
         for (uint32_t i = lane; i < dk; i += 32) {
-            const float x = to_float(qp[i]), y = to_float(kp[i]);
+            const float x = keyq[1][i], y = keyq[0][i];
             qq = fmaf(x, x, qq), kk = fmaf(y, y, kk), qk = fmaf(x, y, qk);
         }
         for (int o = 16; o; o >>= 1) {
@@ -95,18 +110,25 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) k_delta_tick(const __grid
             qk += __shfl_xor_sync(~0u, qk, o);
         }
         float rq = 1.0f, rk = 1.0f;
-        if (c.flags & MDN_DELTA_NORMALIZE) rq = 1.0f / sqrtf(qq + c.norm_eps), rk = 1.0f / sqrtf(kk + c.norm_eps);
-        float ks[V] = {}, qs[V] = {};
+        if (c.flags & MDN_DELTA_NORMALIZE) rq = unit_factor(qq + c.norm_eps), rk = unit_factor(kk + c.norm_eps);
+        float ks[V] = {}, qs[V] = {}, k[NI];
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const uint32_t r = rg + i * nrg;
-            const float kr = r < dk ? to_float(kp[r]) : 0.0f, qr = r < dk ? to_float(qp[r]) : 0.0f;
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                S[i][e] *= a;
-                ks[e] = fmaf(kr, S[i][e], ks[e]);
-                qs[e] = fmaf(qr, S[i][e], qs[e]);
+        for (int i = 0; i < NI; i += 4) {
+            float4 kr = make_float4(0.0f, 0.0f, 0.0f, 0.0f), qr = kr;
+            if (r0 + i < kWide) {
+                kr = *reinterpret_cast<const float4*>(&keyq[0][r0 + i]);
+                qr = *reinterpret_cast<const float4*>(&keyq[1][r0 + i]);
             }
+            const float q[4] = {qr.x, qr.y, qr.z, qr.w};
+            k[i] = kr.x, k[i + 1] = kr.y, k[i + 2] = kr.z, k[i + 3] = kr.w;
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    S[i + n][e] *= a;
+                    ks[e] = fmaf(k[i + n], S[i + n][e], ks[e]);
+                    qs[e] = fmaf(q[n], S[i + n][e], qs[e]);
+                }
         }
         for (int o = 16; o >= (1 << log_cp); o >>= 1) {
 #pragma unroll
@@ -137,28 +159,24 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) k_delta_tick(const __grid
         for (int e = 0; e < V; e++) {
             u[e] = b * (v[e] - rk * ks[e]);
             const float o = c.scale * rq * fmaf(qk * rk, u[e], qs[e]);
-            if (mine && rg == 0) store(row_ptr<T>(c.out, 0, env, head) + col + e, o);
+            if (mine && r0 == 0) store(row_ptr<T>(c.out, 0, env, head) + col + e, o);
             u[e] *= rk;
         }
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const uint32_t r = rg + i * nrg;
-            const float kr = r < dk ? to_float(kp[r]) : 0.0f;
+        for (int i = 0; i < NI; i++)
 #pragma unroll
-            for (int e = 0; e < V; e++) S[i][e] = fmaf(kr, u[e], S[i][e]);
-        }
-    } else if (mine && rg == 0) {
+            for (int e = 0; e < V; e++) S[i][e] = fmaf(k[i], u[e], S[i][e]);
+    } else if (mine && r0 == 0) {
 #pragma unroll
         for (int e = 0; e < V; e++) store(row_ptr<T>(c.out, 0, env, head) + col + e, 0.0f);
     }
-    if (!c.state_out) return;
+    if (!c.state_out || !mine) return;
+    float* d = c.state_out + state + size_t(r0) * dv + col;
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-        const uint32_t r = rg + i * nrg;
-        if (!mine || r >= dk) continue;
-        float* p = c.state_out + state + size_t(r) * dv + col;
-        if constexpr (V == 4) __stcs(reinterpret_cast<float4*>(p), make_float4(S[i][0], S[i][1], S[i][2], S[i][3]));
-        else *p = S[i][0];
+    for (int i = 0; i < NI; i++, d += dv) {
+        if (r0 + i >= dk) break;
+        if constexpr (V == 4) __stcs(reinterpret_cast<float4*>(d), make_float4(S[i][0], S[i][1], S[i][2], S[i][3]));
+        else __stcs(d, S[i][0]);
     }
 }
 
@@ -295,18 +313,12 @@ __device__ __forceinline__ void cp_async_wait() {
 struct ChunkMeta {
     uint32_t t, n;   // first step, steps (0: an item without any)
     uint32_t flags;
-    uint32_t item;
+    uint32_t bh;     // environment x heads + head
+    uint32_t env, head, qh, v0;
 };
 constexpr uint32_t kFresh = 1, kFirst = 2, kLast = 4, kDone = 8;  // an episode starts at t; the item's first, last chunk
 
-struct Item {
-    uint32_t bh, env, head, qh, v0;  // bh: environment x heads + head
-};
 __host__ __device__ inline uint32_t value_blocks(const mdn_delta& c) { return (c.value_dim + 63) / 64; }
-__device__ __forceinline__ Item item_of(const mdn_delta& c, uint32_t item) {
-    const uint32_t blocks = value_blocks(c), bh = item / blocks, env = bh / c.heads, head = bh - env * c.heads;
-    return Item{bh, env, head, head / (c.heads / c.qk_heads), (item - bh * blocks) * 64};
-}
 
 // Walks the chunks of items first, first + stride, ... in order: cells of 16
 // steps, cut at episode starts. One warp holds it; the next cell's start flags
@@ -314,8 +326,8 @@ __device__ __forceinline__ Item item_of(const mdn_delta& c, uint32_t item) {
 struct ChunkWalk {
     const uint8_t* starts;
     uint32_t item, items, stride, live, cell_t, pos, mask, next_flag;
+    uint32_t bh, env, head, qh, v0;
     bool open;  // inside an item
-    Item at;
     __device__ void begin(uint32_t first, uint32_t items_, uint32_t stride_) {
         item = first, items = items_, stride = stride_, open = false;
     }
@@ -323,20 +335,22 @@ struct ChunkWalk {
         return starts && lane < kCell && t + lane < live ? starts[int64_t(t + lane) * c.starts_step] : 0u;
     }
     __device__ ChunkMeta next(const mdn_delta& c, uint32_t lane) {
-        ChunkMeta m{0, 0, 0, item};
+        uint32_t flags = 0;
         if (!open) {
-            if (item >= items) return ChunkMeta{0, 0, kDone, 0};
-            at = item_of(c, item);
-            live = live_steps(c, at.env);
-            starts = c.starts ? c.starts + int64_t(at.env) * c.starts_env : nullptr;
+            if (item >= items) return ChunkMeta{0, 0, kDone};
+            const uint32_t blocks = value_blocks(c);
+            bh = item / blocks, env = bh / c.heads, head = bh - env * c.heads;
+            qh = head / (c.heads / c.qk_heads), v0 = (item - bh * blocks) * 64;
+            live = live_steps(c, env);
+            starts = c.starts ? c.starts + int64_t(env) * c.starts_env : nullptr;
             cell_t = pos = 0;
             const uint32_t now = flag(c, 0, lane);
             next_flag = flag(c, kCell, lane);
             mask = __ballot_sync(~0u, now);
             open = true;
-            m.flags = kFirst;
+            flags = kFirst;
         }
-        m.t = cell_t + pos;
+        ChunkMeta m{cell_t + pos, 0, flags, bh, env, head, qh, v0};
         if (live) {
             const uint32_t later = mask & ~((2u << pos) - 1);
             uint32_t end = later ? __ffs(later) - 1 : kCell;
@@ -360,43 +374,64 @@ struct ChunkWalk {
     }
 };
 
-// n <= 16 rows of `dim` values from step t on into shared rows of ROW bytes,
+// Rows off 16-byte boundaries, value by value; out of line, as the instructions
+// that an SM has at hand are what the rollout kernel runs short of.
+template <class T>
+__device__ __noinline__ void fetch_singles(const T* base, int64_t step, uint32_t dim, uint32_t n, char* dst,
+                                           uint32_t width, uint32_t row, uint32_t lane) {
+    for (uint32_t e = lane; e < kCell * width; e += 32) {
+        const uint32_t r = e / width, col = e % width;
+        T x = T(0.0f);
+        if (r < n && col < dim) x = base[int64_t(r) * step + col];
+        *reinterpret_cast<T*>(dst + r * row + col * sizeof(T)) = x;
+    }
+}
+
+// n <= 16 rows of `dim` values from `base` on into shared rows of ROW bytes,
 // WIDTH values wide; what lies past `dim` or past the rows is zeros.
 template <class T, int WIDTH, int ROW>
-__device__ __forceinline__ void fetch_rows(const mdn_rows& src, bool vec, uint32_t t, uint32_t env, uint32_t head,
-                                           uint32_t first, uint32_t dim, uint32_t n, char* dst, uint32_t lane) {
-    const T* base = row_ptr<T>(src, t, env, head) + first;
+__device__ __forceinline__ void fetch_rows(const T* base, int64_t step, bool vec, uint32_t dim, uint32_t n, char* dst,
+                                           uint32_t lane) {
     if (vec) {
         constexpr uint32_t per = 16 / sizeof(T), granules = WIDTH / per, rows = 32 / granules;
         const uint32_t r0 = lane / granules, col = lane % granules * per;
         const uint32_t bytes = col < dim ? min(per, dim - col) * uint32_t(sizeof(T)) : 0u;
-        const T* p = base + int64_t(r0) * src.step + col;
-        uint32_t d = smem_addr(dst) + r0 * ROW + lane % granules * 16;
+        const T* p = bytes ? base + int64_t(r0) * step + col : base;
+        const int64_t jump = rows * step;
+        const uint32_t d = smem_addr(dst) + r0 * ROW + lane % granules * 16;
 #pragma unroll
         for (uint32_t r = 0; r < kCell; r += rows) {
             const uint32_t got = r0 + r < n ? bytes : 0u;
-            cp_async16(d, got ? p : base, got);
-            p += rows * src.step;
-            d += rows * ROW;
+            cp_async16(d + r * ROW, got ? p : base, got);
+            p += jump;
         }
     } else {
-        for (uint32_t e = lane; e < kCell * WIDTH; e += 32) {
-            const uint32_t r = e / WIDTH, col = e % WIDTH;
-            T x = T(0.0f);
-            if (r < n && col < dim) x = base[int64_t(r) * src.step + col];
-            *reinterpret_cast<T*>(dst + r * ROW + col * sizeof(T)) = x;
-        }
+        fetch_singles(base, step, dim, n, dst, WIDTH, ROW, lane);
     }
 }
 
 // log_decay and beta of a chunk's steps into shared memory; zeros past n.
-__device__ __forceinline__ void fetch_scalars(const mdn_delta& c, uint32_t t, uint32_t env, uint32_t head, uint32_t n,
-                                              float* dst, uint32_t lane) {
-    const mdn_rows& src = lane < kCell ? c.log_decay : c.beta;
+// `p`: of the lane's own array (lanes 0..15: log_decay) at the first step.
+__device__ __forceinline__ void fetch_scalars(const float* p, int64_t step, uint32_t n, float* dst, uint32_t lane) {
     const uint32_t r = lane & (kCell - 1);
-    const float* p = row_ptr<float>(src, t, env, head);
-    cp_async4(smem_addr(dst + lane), r < n ? p + int64_t(r) * src.step : p, r < n ? 4 : 0);
+    cp_async4(smem_addr(dst + lane), r < n ? p + int64_t(r) * step : p, r < n ? 4 : 0);
 }
+
+// Where an environment and head's rows begin.
+template <class T>
+struct Bases {
+    const T *q, *k, *v;
+    const float* scalars;  // log_decay in lanes 0..15, beta in lanes 16..31
+    int64_t scalars_step;
+    __device__ __forceinline__ void set(const mdn_delta& c, uint32_t env, uint32_t head, uint32_t qh, uint32_t v0,
+                                        uint32_t lane) {
+        q = row_ptr<T>(c.q, 0, env, qh);
+        k = row_ptr<T>(c.k, 0, env, qh);
+        v = row_ptr<T>(c.v, 0, env, head) + v0;
+        scalars = row_ptr<float>(lane < kCell ? c.log_decay : c.beta, 0, env, head);
+        scalars_step = lane < kCell ? c.log_decay.step : c.beta.step;
+    }
+};
 
 // 16 rows of DK values (of type T, rows of raw_row bytes) as bf16 parts.
 template <int DK, int ROW>
@@ -445,7 +480,7 @@ __device__ __forceinline__ void key_products(const char* keys, const char* queri
                                              float* squares, uint32_t lane) {
     const uint32_t g = lane >> 2, t = lane & 3, qp = smem_addr(queries), kp = smem_addr(keys);
     float dk0[4] = {}, dk1[4] = {}, dq0[4] = {}, dq1[4] = {}, qq0[4] = {}, qq1[4] = {};
-#pragma unroll
+#pragma unroll 1
     for (int kb = 0; kb < DK / 16; kb++) {
         uint32_t ak[NP][4], bk[NP][4], bq[NP][4];
 #pragma unroll
@@ -478,12 +513,6 @@ __device__ __forceinline__ void key_products(const char* keys, const char* queri
     }
 }
 
-// 1 / sqrt(x), the hardware's estimate with a Newton step.
-__device__ __forceinline__ float unit_factor(float x) {
-    const float r = rsqrtf(x);
-    return x > 0.0f && r > 0.0f ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
-}
-
 // Column j of (I + A)^-1 by forward substitution, each step's value subtracted
 // from all later ones. `cols`: A as [j][i].
 __device__ __forceinline__ void substitute(float (&col)[16], const float* cols, uint32_t j) {
@@ -510,10 +539,9 @@ __device__ __forceinline__ void store_parts(float (&col)[16], char* dst) {
     }
 }
 
-// The forward kernel's stages, each a warp's work on a chunk of its own while
-// four warps compute chunk i: one fetches chunk i + kLead and finishes the
-// matrices of chunk i + 1, one starts those of chunk i + 2. Rows live in rings
-// of slots. i is the step that reads, j the step that wrote: c (I + A)^-1 is
+// The forward kernel's stages, each on a chunk of its own while four warps
+// compute chunk i: one warp fetches chunk i + kLead and finishes the matrices of
+// chunk i + 1, one starts those of chunk i + 2. Rows live in rings of slots. i is the step that reads, j the step that wrote: c (I + A)^-1 is
 // kept as [j][i], P (I + A)^-1 as [i][j].
 template <class T, int DK>
 struct Forward {
@@ -525,7 +553,7 @@ struct Forward {
     static constexpr int kRawRow = DK * int(sizeof(T)) + 16;
     static constexpr int kRawV = 64 * int(sizeof(T)) + 16;
     static constexpr int kKeys = 2 * kCell * kRawRow;           // queries, keys
-    static constexpr int kSlotS = kCell * kRawV, kSlot = kSlotS + 128 + 16;  // values, 16 log-decays and betas, ChunkMeta
+    static constexpr int kSlotS = kCell * kRawV, kSlot = kSlotS + 128 + 32;  // values, 16 log-decays and betas, ChunkMeta
     static constexpr int kStageK = kParts == 3 ? 3 * kCell * kRow : 0;  // after the queries' parts
     static constexpr int kStageT = 2 * kStageK;                 // three parts of c (I + A)^-1, then of P (I + A)^-1
     static constexpr int kStageP = kStageT + 3 * kCell * kMatRow;
@@ -552,20 +580,22 @@ struct Forward {
     __device__ const char* queries(uint32_t i) const { return kParts == 1 ? rows(i) : stage(i); }
     __device__ const char* keys(uint32_t i) const { return kParts == 1 ? rows(i) + kCell * kRawRow : stage(i) + kStageK; }
 
-    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, const Item& at, uint32_t i,
+    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, const Bases<T>& at, uint32_t i,
                           uint32_t lane) const {
         char* dst = slot(i);
         if (lane == 0) *meta(i) = m;
         if (m.n) {
-            fetch_rows<T, DK, kRawRow>(c.q, vec & 1, m.t, at.env, at.qh, 0, c.key_dim, m.n, rows(i), lane);
-            fetch_rows<T, DK, kRawRow>(c.k, vec & 2, m.t, at.env, at.qh, 0, c.key_dim, m.n, rows(i) + kCell * kRawRow,
-                                       lane);
-            fetch_rows<T, 64, kRawV>(c.v, vec & 4, m.t, at.env, at.head, at.v0, min(64u, c.value_dim - at.v0), m.n, dst,
-                                     lane);
-            fetch_scalars(c, m.t, at.env, at.head, m.n, reinterpret_cast<float*>(dst + kSlotS), lane);
+            char* key_rows = rows(i);
+            fetch_rows<T, DK, kRawRow>(at.q + int64_t(m.t) * c.q.step, c.q.step, vec & 1, c.key_dim, m.n, key_rows, lane);
+            fetch_rows<T, DK, kRawRow>(at.k + int64_t(m.t) * c.k.step, c.k.step, vec & 2, c.key_dim, m.n,
+                                       key_rows + kCell * kRawRow, lane);
+            fetch_rows<T, 64, kRawV>(at.v + int64_t(m.t) * c.v.step, c.v.step, vec & 4, min(64u, c.value_dim - m.v0), m.n,
+                                     dst, lane);
+            fetch_scalars(at.scalars + int64_t(m.t) * at.scalars_step, at.scalars_step, m.n,
+                          reinterpret_cast<float*>(dst + kSlotS), lane);
         }
         if (m.flags & kFirst && c.state_in && !(m.flags & kFresh)) {  // the state, on its way to the L2 cache
-            const char* p = reinterpret_cast<const char*>(c.state_in + size_t(at.bh) * c.key_dim * c.value_dim);
+            const char* p = reinterpret_cast<const char*>(c.state_in + size_t(m.bh) * c.key_dim * c.value_dim);
             const uint32_t bytes = c.key_dim * c.value_dim * 4;
             for (uint32_t b = lane * 128; b < bytes; b += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
         }
@@ -689,7 +719,13 @@ struct Forward {
     }
 };
 
-// Values of two value columns (col, col + 1) of one step.
+// Values of two value columns (col, col + 1) of one step; apart where rows are
+// not on pairs' boundaries, or have no second.
+template <class T>
+__device__ __forceinline__ void store_apart(T* p, uint32_t col, uint32_t cols, float x, float y) {
+    if (col < cols) store(p + col, x);
+    if (col + 1 < cols) store(p + col + 1, y);
+}
 template <class T>
 __device__ __forceinline__ void store_two(T* p, bool pair, uint32_t col, uint32_t cols, float x, float y) {
     if (pair) {
@@ -697,8 +733,7 @@ __device__ __forceinline__ void store_two(T* p, bool pair, uint32_t col, uint32_
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p + col) = make_float2(x, y);
         else *reinterpret_cast<uint32_t*>(p + col) = round_pair(x, y);
     } else {
-        if (col < cols) store(p + col, x);
-        if (col + 1 < cols) store(p + col + 1, y);
+        store_apart(p, col, cols, x, y);
     }
 }
 
@@ -715,6 +750,7 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
     if (warp == warps + 1) {
         ChunkWalk walk;
         walk.begin(blockIdx.x, items, gridDim.x);
+        Bases<T> at;
         for (int i = -F::kLead;; i++) {
             if (i >= 0 && f.meta(i)->flags & kDone) break;
             if constexpr (NP == 3) {
@@ -724,7 +760,8 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
                 }
             }
             const ChunkMeta m = walk.next(c, lane);
-            f.fetch(c, vec, m, walk.at, i + F::kLead, lane);
+            if (m.flags & kFirst) at.set(c, m.env, m.head, m.qh, m.v0, lane);
+            f.fetch(c, vec, m, at, i + F::kLead, lane);
             if (i + 1 >= 0 && f.meta(i + 1)->n) f.finish(i + 1, lane);
             cp_async_wait<F::kPending>();
             __syncthreads();
@@ -750,9 +787,8 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
     for (uint32_t i = 0;; i++) {
         const ChunkMeta m = *f.meta(i);
         if (m.flags & kDone) break;
-        const Item at = item_of(c, m.item);
-        const uint32_t col = at.v0 + colw;
-        const size_t state = size_t(at.bh) * c.key_dim * dv;
+        const uint32_t col = m.v0 + colw;
+        const size_t state = size_t(m.bh) * c.key_dim * dv;
         if (m.flags & (kFirst | kFresh)) {
             const bool read = c.state_in && !(m.flags & kFresh);
 #pragma unroll
@@ -777,7 +813,7 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
             const float* fac = reinterpret_cast<const float*>(st + F::kStageVec);
             if (c.saved && m.t % kCell == 0 && col < dvp) {
                 float* d = static_cast<float*>(c.saved) +
-                           (size_t(m.t / kCell) * c.envs * c.heads + at.bh) * c.key_dim * dvp + col;
+                           (size_t(m.t / kCell) * c.envs * c.heads + m.bh) * c.key_dim * dvp + col;
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -835,7 +871,7 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
             for (int p = 0; p < 3; p++)
                 ldsm4(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
             mma_parts<3, 3>(o[0], o[1], parts, b);
-            T* out = row_ptr<T>(c.out, m.t, at.env, at.head);
+            T* out = row_ptr<T>(c.out, m.t, m.env, m.head);
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -864,8 +900,8 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
             }
         }
         if (m.flags & kLast) {
-            for (uint32_t t = m.t + m.n; t < c.steps; t++)
-                if (t4 == 0) store_two(row_ptr<T>(c.out, t, at.env, at.head), false, col, dv, 0.0f, 0.0f);
+            for (uint32_t t = m.t + m.n + t4; t < c.steps; t += 4)
+                store_two(row_ptr<T>(c.out, t, m.env, m.head), vec & 8, col, dv, 0.0f, 0.0f);
             if (c.state_out) {
 #pragma unroll
                 for (int j = 0; j < NT; j++)
@@ -930,10 +966,10 @@ struct ChunkWalkBack {
         return starts && lane < kCell && t + lane < live ? starts[int64_t(t + lane) * starts_step] : 0u;
     }
     __device__ ChunkMeta next(uint32_t lane) {
-        if (done) return ChunkMeta{0, 0, kDone, 0};
+        if (done) return ChunkMeta{0, 0, kDone};
         const uint32_t earlier = mask & ((1u << pos) - 1);
         const uint32_t first = earlier ? 31 - __clz(earlier) : 0;
-        const ChunkMeta m{cell_t + first, pos - first, (mask >> first) & 1 ? kFresh : 0u, 0};
+        const ChunkMeta m{cell_t + first, pos - first, (mask >> first) & 1 ? kFresh : 0u};
         pos = first;
         if (pos == 0) {
             done = cell_t == 0;
@@ -956,7 +992,7 @@ struct Backward {
     static constexpr int kRow = DK * 2 + 16, kRowV = 64 * 2 + 16;
     static constexpr int kRawRow = DK * int(sizeof(T)) + 16, kRawV = 64 * int(sizeof(T)) + 16;
     static constexpr int kSlotK = kCell * kRawRow, kSlotV = 2 * kSlotK, kSlotO = kSlotV + kCell * kRawV;
-    static constexpr int kSlotS = kSlotO + kCell * kRawV, kSlot = kSlotS + 128 + 16;
+    static constexpr int kSlotS = kSlotO + kCell * kRawV, kSlot = kSlotS + 128 + 32;
     static constexpr int kMat = 3 * kCell * kMatRow;            // three parts of a 16 x 16 matrix
     static constexpr int kSquare = kCell * kScratchRow * 4;     // a 16 x 16 matrix of floats
     static constexpr int kStageK = kParts == 3 ? 3 * kCell * kRow : 0;
@@ -988,16 +1024,16 @@ struct Backward {
     __device__ const char* douts(uint32_t i) const { return kParts == 1 ? slot(i) + kSlotO : stage(i) + kStageO; }
 
     __device__ void fetch(const mdn_delta& c, const mdn_delta_grads& d, uint32_t vec, const ChunkMeta& m, uint32_t i,
-                          uint32_t env, uint32_t head, uint32_t qh, uint32_t v0, uint32_t lane) const {
+                          const Bases<T>& at, const T* dout, uint32_t dv, uint32_t lane) const {
         char* dst = slot(i);
         if (lane == 0) *meta(i) = m;
         if (m.n) {
-            const uint32_t dv = min(64u, c.value_dim - v0);
-            fetch_rows<T, DK, kRawRow>(c.q, vec & 1, m.t, env, qh, 0, c.key_dim, m.n, dst, lane);
-            fetch_rows<T, DK, kRawRow>(c.k, vec & 2, m.t, env, qh, 0, c.key_dim, m.n, dst + kSlotK, lane);
-            fetch_rows<T, 64, kRawV>(c.v, vec & 4, m.t, env, head, v0, dv, m.n, dst + kSlotV, lane);
-            fetch_rows<T, 64, kRawV>(d.dout, vec & 16, m.t, env, head, v0, dv, m.n, dst + kSlotO, lane);
-            fetch_scalars(c, m.t, env, head, m.n, reinterpret_cast<float*>(dst + kSlotS), lane);
+            fetch_rows<T, DK, kRawRow>(at.q + int64_t(m.t) * c.q.step, c.q.step, vec & 1, c.key_dim, m.n, dst, lane);
+            fetch_rows<T, DK, kRawRow>(at.k + int64_t(m.t) * c.k.step, c.k.step, vec & 2, c.key_dim, m.n, dst + kSlotK, lane);
+            fetch_rows<T, 64, kRawV>(at.v + int64_t(m.t) * c.v.step, c.v.step, vec & 4, dv, m.n, dst + kSlotV, lane);
+            fetch_rows<T, 64, kRawV>(dout + int64_t(m.t) * d.dout.step, d.dout.step, vec & 16, dv, m.n, dst + kSlotO, lane);
+            fetch_scalars(at.scalars + int64_t(m.t) * at.scalars_step, at.scalars_step, m.n,
+                          reinterpret_cast<float*>(dst + kSlotS), lane);
         }
         cp_async_commit();
     }
@@ -1131,23 +1167,27 @@ __global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_d
     if (warp == 5) {
         ChunkWalkBack walk;
         walk.begin(c, env, live, lane);
+        Bases<T> at;
+        at.set(c, env, head, qh, v0, lane);
+        const T* dout = row_ptr<T>(d.dout, 0, env, head) + v0;
+        const uint32_t cols = min(64u, dv - v0);
         if constexpr (F::kAhead) {
-            f.fetch(c, d, vec, walk.next(lane), 0, env, head, qh, v0, lane);
-            f.fetch(c, d, vec, walk.next(lane), 1, env, head, qh, v0, lane);
+            f.fetch(c, d, vec, walk.next(lane), 0, at, dout, cols, lane);
+            f.fetch(c, d, vec, walk.next(lane), 1, at, dout, cols, lane);
             cp_async_wait<0>();
             __syncthreads();
             __syncthreads();
             for (uint32_t i = 0; f.meta(i)->n; i++) {
-                f.fetch(c, d, vec, walk.next(lane), i + 2, env, head, qh, v0, lane);
+                f.fetch(c, d, vec, walk.next(lane), i + 2, at, dout, cols, lane);
                 cp_async_wait<0>();
                 __syncthreads();
             }
         } else {
-            f.fetch(c, d, vec, walk.next(lane), 0, env, head, qh, v0, lane);
+            f.fetch(c, d, vec, walk.next(lane), 0, at, dout, cols, lane);
             cp_async_wait<0>();
             __syncthreads();
             for (uint32_t i = 0; f.meta(i)->n; i++) {
-                f.fetch(c, d, vec, walk.next(lane), i + 1, env, head, qh, v0, lane);
+                f.fetch(c, d, vec, walk.next(lane), i + 1, at, dout, cols, lane);
                 __syncthreads();
                 cp_async_wait<0>();
                 __syncthreads();
@@ -1189,7 +1229,7 @@ __global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_d
         }
     for (uint32_t t = live; t < c.steps; t++) {
         const size_t part = ((size_t(t) * c.envs + env) * c.heads + head) * value_blocks(c) + blockIdx.y;
-        if (t4 == 0) store_two(row_ptr<T>(d.dv, t, env, head), false, col, dv, 0.0f, 0.0f);
+        if (t4 == 0) store_two(row_ptr<T>(d.dv, t, env, head), vec & 8, col, dv, 0.0f, 0.0f);
         for (uint32_t i = threadIdx.x; i < dk; i += 128) {
             if (shared_rows) shares.dq[part * dk + i] = shares.dk[part * dk + i] = 0.0f;
             else store(row_ptr<T>(d.dq, t, env, qh) + i, 0.0f), store(row_ptr<T>(d.dk, t, env, qh) + i, 0.0f);
