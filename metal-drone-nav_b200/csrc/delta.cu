@@ -1245,24 +1245,34 @@ __global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_d
     float* frob = row_sums + 16;
     __syncthreads();
     if constexpr (F::kAhead) __syncthreads();
-    for (uint32_t i = 0;; i++) {
-        const ChunkMeta m = *f.meta(i);
-        if (!m.n) break;
-        // The state before the chunk: zeros after a start inside the cell.
-        const bool cell = m.t % kCell == 0;
-        const float* saved = static_cast<const float*>(c.saved) +
-                             (size_t(m.t / kCell) * c.envs * c.heads + blockIdx.x) * dk * dvp;
-        float S[NT][4];
+    // The states before the chunks: zeros after a start inside a cell. The next
+    // chunk's is on its way while this one is finished.
+    auto saved_at = [&](const ChunkMeta& m) {
+        return static_cast<const float*>(c.saved) + (size_t(m.t / kCell) * c.envs * c.heads + blockIdx.x) * dk * dvp;
+    };
+    float S[NT][4];
+    auto load_state = [&](const ChunkMeta& m) {
+        const float* p = saved_at(m) + size_t(2 * t4) * dvp + col;
+        const bool in = m.n && m.t % kCell == 0 && col < dvp;
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const uint32_t r = 8 * j + 2 * t4 + e;
                 float2 x = make_float2(0.0f, 0.0f);
-                if (cell && r < dk && col < dvp) x = *reinterpret_cast<const float2*>(saved + size_t(r) * dvp + col);
+                if (in && 8 * j + 2 * t4 + e < dk) x = *reinterpret_cast<const float2*>(p + (8 * j + e) * dvp);
                 S[j][e] = x.x, S[j][2 + e] = x.y;
             }
-        if constexpr (!F::kAhead) __syncthreads();
+    };
+    if constexpr (F::kAhead) load_state(*f.meta(0));
+    for (uint32_t i = 0;; i++) {
+        const ChunkMeta m = *f.meta(i);
+        if (!m.n) break;
+        const bool cell = m.t % kCell == 0;
+        const float* saved = saved_at(m);
+        if constexpr (!F::kAhead) {
+            load_state(m);
+            __syncthreads();
+        }
         const char* st = f.stage(i);
         const char* slot = f.slot(i);
         const float* fac = reinterpret_cast<const float*>(st + F::kStageVec);
@@ -1484,6 +1494,21 @@ __global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_d
                 }
             }
         }
+        // this warp's key columns of the state, for after the barrier
+        float2 sx[16];
+        auto load_keys = [&](uint32_t k0) {
+            const float* p = saved + size_t(k0 + g) * dvp + v0 + 2 * t4;
+#pragma unroll
+            for (int vb = 0; vb < 4; vb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t key = k0 + g + 8 * (r >> 1), value = v0 + vb * 16 + 2 * t4 + 8 * (r & 1);
+                    sx[vb * 4 + r] = make_float2(0.0f, 0.0f);
+                    if (cell && key < dk && value < dvp)
+                        sx[vb * 4 + r] = *reinterpret_cast<const float2*>(p + (8 * (r >> 1)) * dvp + vb * 16 + 8 * (r & 1));
+                }
+        };
+        load_keys(warp * 16);
         asm volatile("bar.sync 1, 128;" ::: "memory");
 
         // ---- F and E: the warps' shares together, with their factors
@@ -1542,17 +1567,14 @@ __global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_d
         for (int s = 0; s < NS; s++) {
             const uint32_t k0 = (s * 4 + warp) * 16;
             if (k0 >= DK) break;
+            if (s) load_keys(k0);
 #pragma unroll
             for (int vb = 0; vb < 4; vb++) {
                 uint32_t oa2[NP][4], xa[NO][4], wa[NO][4], sb[NO][4], db[NO][4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const uint32_t key = k0 + g + 8 * (r >> 1), value = v0 + vb * 16 + 2 * t4 + 8 * (r & 1);
-                    float2 x = make_float2(0.0f, 0.0f);
-                    if (cell && key < dk && value < dvp)
-                        x = *reinterpret_cast<const float2*>(saved + size_t(key) * dvp + value);
                     uint32_t p[NO];
-                    cut_pair<NO>(x.x, x.y, p);
+                    cut_pair<NO>(sx[vb * 4 + r].x, sx[vb * 4 + r].y, p);
 #pragma unroll
                     for (int n = 0; n < NO; n++) sb[n][r] = p[n];
                 }
@@ -1570,6 +1592,7 @@ __global__ void __maxnreg__(168) k_delta_gradients(const __grid_constant__ mdn_d
                 mma_out<NO, NO>(aw[s][0], aw[s][1], wa, db);
             }
         }
+        if constexpr (F::kAhead) load_state(*f.meta(i + 1));
         asm volatile("bar.sync 1, 128;" ::: "memory");
 
         // q.dq and k.dk of step lane & 15: column sums of F (k.q) or E (k.k), rows' sums, sums over value columns
