@@ -646,3 +646,18 @@ def test_library_refuses_null_call(mdn):
     assert lib.mdn_delta_forward(None, None) == 1 and b"null call" in lib.mdn_last_error()
     assert lib.mdn_block_norm_forward(None, None) == 1
     assert lib.mdn_delta_saved_bytes(None) == 0
+
+
+def test_example_learns_and_ticks_agree():
+    """The example end to end: the loss falls, and ticks give what the rollout gave. Two runs of the same layers in
+    32 bits, one by rows of a rollout and one by ticks: each within F32_NORM of the exact values, through products that
+    torch may sum in another order (u sqrt(184) = 1e-6 of a value)."""
+    import importlib.util
+
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("memory_policy", ROOT / "examples" / "memory_policy.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, off = example.run(envs=96, horizon=24, rollouts=5, report=lambda line: None)
+    assert losses[-1] < 0.7 * losses[0], losses
+    assert max(off) <= 4 * F32_NORM, off
