@@ -542,6 +542,12 @@ size_t mdn_delta_workspace_bytes(const mdn_delta* call);
 /* One rollout (any number of steps, 0 and 1 among them: one step is the
  * policy tick). steps, envs of 0 are allowed. */
 int mdn_delta_forward(const mdn_delta* call, void* stream);
+/* The same with a workspace (mdn_delta_forward_bytes bytes, 16-byte aligned;
+ * 0 for most shapes): a long rollout of few environments is then cut into
+ * segments that run at once and are joined. NULL = never cut. The results
+ * differ in rounding alone. */
+size_t mdn_delta_forward_bytes(const mdn_delta* call);
+int mdn_delta_forward_with(const mdn_delta* call, void* workspace, void* stream);
 /* Its gradients. `call` as it was given to mdn_delta_forward, with `saved`
  * filled by that call; its out and state_out are not read. Deterministic:
  * sums over a group's heads are taken in a fixed order. */

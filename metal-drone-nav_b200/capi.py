@@ -91,6 +91,8 @@ SIGNATURES = {
                                                  ctypes.c_float, _P]),
     "mdn_delta_saved_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
     "mdn_delta_workspace_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
+    "mdn_delta_forward_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
+    "mdn_delta_forward_with": (ctypes.c_int, [ctypes.c_char_p, _P, _P]),
     "mdn_delta_forward": (ctypes.c_int, [ctypes.c_char_p, _P]),
     "mdn_delta_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _P]),
     "mdn_block_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),

@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <string>
@@ -316,7 +317,23 @@ struct ChunkMeta {
     uint32_t bh;     // environment x heads + head
     uint32_t env, head, qh, v0;
 };
-constexpr uint32_t kFresh = 1, kFirst = 2, kLast = 4, kDone = 8;  // an episode starts at t; the item's first, last chunk
+// An episode starts at t; the item's first, last chunk; the end of the stream;
+// an item of the segment's map. From bit 8 on: the segment.
+constexpr uint32_t kFresh = 1, kFirst = 2, kLast = 4, kDone = 8, kMap = 16;
+
+// A long rollout of few environments is cut into segments of `cells` cells that
+// run at once. A chunk is linear in the state it begins with, so a segment is
+// S -> M S + b: pass kJoin runs every segment but the last from zeros (its last
+// state is b) and, on no values, from the unit matrix (its last state is M, as
+// columns of a memory of key_dim values); k_delta_carry goes through them for
+// the state that each segment begins with; pass kRun computes the outputs.
+// Twice to three times the work, over so many more SMs.
+enum Pass : uint32_t { kRun = 0, kJoin = 1 };
+struct Segments {
+    uint32_t count, cells;
+    Pass pass;
+    float *carry, *map;  // [count - 1][envs x heads][key][value], [..][key][key]
+};
 
 __host__ __device__ inline uint32_t value_blocks(const mdn_delta& c) { return (c.value_dim + 63) / 64; }
 
@@ -326,7 +343,7 @@ __host__ __device__ inline uint32_t value_blocks(const mdn_delta& c) { return (c
 struct ChunkWalk {
     const uint8_t* starts;
     uint32_t item, items, stride, live, cell_t, pos, mask, next_flag;
-    uint32_t bh, env, head, qh, v0;
+    uint32_t bh, env, head, qh, v0, kind;
     bool open;  // inside an item
     __device__ void begin(uint32_t first, uint32_t items_, uint32_t stride_) {
         item = first, items = items_, stride = stride_, open = false;
@@ -334,24 +351,39 @@ struct ChunkWalk {
     __device__ uint32_t flag(const mdn_delta& c, uint32_t t, uint32_t lane) const {
         return starts && lane < kCell && t + lane < live ? starts[int64_t(t + lane) * c.starts_step] : 0u;
     }
-    __device__ ChunkMeta next(const mdn_delta& c, uint32_t lane) {
-        uint32_t flags = 0;
+    template <bool SPLIT>
+    __device__ ChunkMeta next(const mdn_delta& c, const Segments& g, uint32_t lane) {
+        uint32_t first = 0;
         if (!open) {
             if (item >= items) return ChunkMeta{0, 0, kDone};
-            const uint32_t blocks = value_blocks(c);
-            bh = item / blocks, env = bh / c.heads, head = bh - env * c.heads;
-            qh = head / (c.heads / c.qk_heads), v0 = (item - bh * blocks) * 64;
+            const uint32_t values = value_blocks(c);
+            const uint32_t blocks = SPLIT && g.pass == kJoin ? values + (c.key_dim + 63) / 64 : values;
+            uint32_t rest = item;
+            kind = cell_t = 0;
+            if constexpr (SPLIT) {
+                const uint32_t all = c.envs * c.heads * blocks, segment = item / all;
+                rest -= segment * all;
+                kind = segment << 8;
+                cell_t = segment * g.cells * kCell;
+            }
+            bh = rest / blocks, env = bh / c.heads, head = bh - env * c.heads;
+            qh = head / (c.heads / c.qk_heads), v0 = rest - bh * blocks;
             live = live_steps(c, env);
+            if constexpr (SPLIT) {
+                if (v0 >= values) kind |= kMap, v0 -= values;
+                if ((kind >> 8) + 1 < g.count) live = min(live, cell_t + g.cells * kCell);
+            }
+            v0 *= 64;
             starts = c.starts ? c.starts + int64_t(env) * c.starts_env : nullptr;
-            cell_t = pos = 0;
-            const uint32_t now = flag(c, 0, lane);
-            next_flag = flag(c, kCell, lane);
+            pos = 0;
+            const uint32_t now = flag(c, cell_t, lane);
+            next_flag = flag(c, cell_t + kCell, lane);
             mask = __ballot_sync(~0u, now);
             open = true;
-            flags = kFirst;
+            first = kFirst;
         }
-        ChunkMeta m{cell_t + pos, 0, flags, bh, env, head, qh, v0};
-        if (live) {
+        ChunkMeta m{cell_t + pos, 0, kind | first, bh, env, head, qh, v0};
+        if (cell_t + pos < live) {
             const uint32_t later = mask & ~((2u << pos) - 1);
             uint32_t end = later ? __ffs(later) - 1 : kCell;
             end = min(end, live - cell_t);
@@ -580,8 +612,9 @@ struct Forward {
     __device__ const char* queries(uint32_t i) const { return kParts == 1 ? rows(i) : stage(i); }
     __device__ const char* keys(uint32_t i) const { return kParts == 1 ? rows(i) + kCell * kRawRow : stage(i) + kStageK; }
 
-    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, const Bases<T>& at, uint32_t i,
-                          uint32_t lane) const {
+    // values: the value columns to fetch
+    __device__ void fetch(const mdn_delta& c, uint32_t vec, const ChunkMeta& m, const Bases<T>& at, uint32_t values,
+                          uint32_t i, uint32_t lane) const {
         char* dst = slot(i);
         if (lane == 0) *meta(i) = m;
         if (m.n) {
@@ -589,12 +622,12 @@ struct Forward {
             fetch_rows<T, DK, kRawRow>(at.q + int64_t(m.t) * c.q.step, c.q.step, vec & 1, c.key_dim, m.n, key_rows, lane);
             fetch_rows<T, DK, kRawRow>(at.k + int64_t(m.t) * c.k.step, c.k.step, vec & 2, c.key_dim, m.n,
                                        key_rows + kCell * kRawRow, lane);
-            fetch_rows<T, 64, kRawV>(at.v + int64_t(m.t) * c.v.step, c.v.step, vec & 4, min(64u, c.value_dim - m.v0), m.n,
-                                     dst, lane);
+            fetch_rows<T, 64, kRawV>(at.v + int64_t(m.t) * c.v.step, c.v.step, vec & 4,
+                                     values, m.n, dst, lane);
             fetch_scalars(at.scalars + int64_t(m.t) * at.scalars_step, at.scalars_step, m.n,
                           reinterpret_cast<float*>(dst + kSlotS), lane);
         }
-        if (m.flags & kFirst && c.state_in && !(m.flags & kFresh)) {  // the state, on its way to the L2 cache
+        if (m.flags & kFirst && c.state_in && !(m.flags & kFresh) && m.flags < 256) {  // the state, on its way to the L2 cache
             const char* p = reinterpret_cast<const char*>(c.state_in + size_t(m.bh) * c.key_dim * c.value_dim);
             const uint32_t bytes = c.key_dim * c.value_dim * 4;
             for (uint32_t b = lane * 128; b < bytes; b += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
@@ -739,12 +772,13 @@ __device__ __forceinline__ void store_two(T* p, bool pair, uint32_t col, uint32_
 
 // A CTA takes 64 value columns of one environment and head after the other; a
 // warp for each 16 of them.
-template <class T, int DK>
+template <class T, int DK, bool SPLIT>
 __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_constant__ mdn_delta c, uint32_t vec,
-                                                                 uint32_t items) {
+                                                                 uint32_t items, const __grid_constant__ Segments seg) {
     using F = Forward<T, DK>;
     constexpr int NP = F::kParts, NT = DK / 8;
     extern __shared__ __align__(16) char smem_raw[];
+    const bool join = SPLIT && seg.pass == kJoin;
     const F f(smem_raw);
     const uint32_t warps = blockDim.x / 32 - 2, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == warps + 1) {
@@ -759,9 +793,9 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
                     asm volatile("bar.sync 2, 64;" ::: "memory");
                 }
             }
-            const ChunkMeta m = walk.next(c, lane);
-            if (m.flags & kFirst) at.set(c, m.env, m.head, m.qh, m.v0, lane);
-            f.fetch(c, vec, m, at, i + F::kLead, lane);
+            const ChunkMeta m = walk.template next<SPLIT>(c, seg, lane);
+            if (m.flags & kFirst) at.set(c, m.env, m.head, m.qh, SPLIT && m.flags & kMap ? 0 : m.v0, lane);
+            f.fetch(c, vec, m, at, SPLIT && m.flags & kMap ? 0u : min(64u, c.value_dim - m.v0), i + F::kLead, lane);
             if (i + 1 >= 0 && f.meta(i + 1)->n) f.finish(i + 1, lane);
             cp_async_wait<F::kPending>();
             __syncthreads();
@@ -789,15 +823,20 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
         if (m.flags & kDone) break;
         const uint32_t col = m.v0 + colw;
         const size_t state = size_t(m.bh) * c.key_dim * dv;
+        const uint32_t segment = SPLIT ? m.flags >> 8 : 0;
+        const size_t all = size_t(c.envs) * c.heads * c.key_dim;  // rows of a segment's states
         if (m.flags & (kFirst | kFresh)) {
-            const bool read = c.state_in && !(m.flags & kFresh);
+            const bool unit = SPLIT && m.flags & kMap && !(m.flags & kFresh);
+            const float* from = join || m.flags & kFresh ? nullptr
+                                : segment               ? seg.carry + (segment - 1) * all * dv
+                                                        : c.state_in;
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const uint32_t r = 8 * j + 2 * t4 + e;
-                    const float* p = c.state_in + state + size_t(r) * dv + col;
-                    const bool in = read && r < c.key_dim;
+                    const float* p = from + state + size_t(r) * dv + col;
+                    const bool in = from && r < c.key_dim;
                     float2 x = make_float2(0.0f, 0.0f);
                     if (vec & 128) {
                         if (in && col < dv) x = *reinterpret_cast<const float2*>(p);
@@ -805,13 +844,14 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
                         if (in && col < dv) x.x = p[0];
                         if (in && col + 1 < dv) x.y = p[1];
                     }
+                    if (SPLIT && unit) x = make_float2(r == col ? 1.0f : 0.0f, r == col + 1 ? 1.0f : 0.0f);
                     S[j][e] = x.x, S[j][2 + e] = x.y;
                 }
         }
         if (m.n) {
             const char* st = f.stage(i);
             const float* fac = reinterpret_cast<const float*>(st + F::kStageVec);
-            if (c.saved && m.t % kCell == 0 && col < dvp) {
+            if (c.saved && !join && m.t % kCell == 0 && col < dvp) {
                 float* d = static_cast<float*>(c.saved) +
                            (size_t(m.t / kCell) * c.envs * c.heads + m.bh) * c.key_dim * dvp + col;
 #pragma unroll
@@ -833,11 +873,11 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
                     ldsm4(bk[p], kp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
-                    ldsm4(bq[p], qp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
+                    if (!join) ldsm4(bq[p], qp + p * kCell * F::kRow + kb * 32 + lane_cols_first(lane, F::kRow));
                 }
                 cut_tiles<3>(S[2 * kb], S[2 * kb + 1], a);
                 mma_parts<3, NP>(xk[0], xk[1], ek[0], ek[1], a, bk);
-                mma_parts<3, NP>(xq[0], xq[1], eq[0], eq[1], a, bq);
+                if (!join) mma_parts<3, NP>(xq[0], xq[1], eq[0], eq[1], a, bq);
             }
             // X = V - g K S, and g Q S
 #pragma unroll
@@ -867,20 +907,22 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
             for (int p = 0; p < 3; p++)
                 ldsm4t(b[p], smem_addr(st + F::kStageT) + p * kCell * kMatRow + lane_rows_first(lane, kMatRow));
             mma_parts<3, 3>(u[0], u[1], parts, b);
+            if (!join) {
 #pragma unroll
-            for (int p = 0; p < 3; p++)
-                ldsm4(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
-            mma_parts<3, 3>(o[0], o[1], parts, b);
-            T* out = row_ptr<T>(c.out, m.t, m.env, m.head);
+                for (int p = 0; p < 3; p++)
+                    ldsm4(b[p], smem_addr(st + F::kStageP) + p * kCell * kMatRow + lane_cols_first(lane, kMatRow));
+                mma_parts<3, 3>(o[0], o[1], parts, b);
+                T* out = row_ptr<T>(c.out, m.t, m.env, m.head);
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+                for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t s = 8 * n + 2 * t4 + e;
-                    if (s < m.n)
-                        store_two(out + int64_t(s) * c.out.step, vec & 8, col, dv, o[n][e] + xq[n][e],
-                                  o[n][2 + e] + xq[n][2 + e]);
-                }
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t s = 8 * n + 2 * t4 + e;
+                        if (s < m.n)
+                            store_two(out + int64_t(s) * c.out.step, vec & 8, col, dv, o[n][e] + xq[n][e],
+                                      o[n][2 + e] + xq[n][2 + e]);
+                    }
+            }
             // S' = g_C S + (c W)^T K
             cut_tiles<3>(u[0], u[1], parts);
             const float gc = fac[48];
@@ -900,20 +942,81 @@ __global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_c
             }
         }
         if (m.flags & kLast) {
-            for (uint32_t t = m.t + m.n + t4; t < c.steps; t += 4)
-                store_two(row_ptr<T>(c.out, t, m.env, m.head), vec & 8, col, dv, 0.0f, 0.0f);
-            if (c.state_out) {
+            float* to = c.state_out;
+            uint32_t width = dv;
+            if (join) {
+                width = m.flags & kMap ? c.key_dim : dv;
+                to = (m.flags & kMap ? seg.map : seg.carry) + segment * all * width;
+            } else {
+                const bool last = !SPLIT || segment + 1 == seg.count;
+                const uint32_t end = last ? c.steps : (segment + 1) * seg.cells * kCell;
+                for (uint32_t t = m.t + m.n + t4; t < end; t += 4)
+                    store_two(row_ptr<T>(c.out, t, m.env, m.head), vec & 8, col, dv, 0.0f, 0.0f);
+                if (!last) to = nullptr;
+            }
+            if (to) {
+                to += size_t(m.bh) * c.key_dim * width;
+                const bool pair = join ? width % 2 == 0 : (vec & 128) != 0;
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const uint32_t r = 8 * j + 2 * t4 + e;
-                        if (r < c.key_dim)
-                            store_two(c.state_out + state + size_t(r) * dv, vec & 128, col, dv, S[j][e], S[j][2 + e]);
+                        if (r < c.key_dim) store_two(to + size_t(r) * width, pair, col, width, S[j][e], S[j][2 + e]);
                     }
             }
         }
         __syncthreads();
+    }
+}
+
+// The state that each segment but the first begins with, over its b: 16 value
+// columns of one environment and head a block, four of them of one key row a
+// thread. A map's zeros take nothing with them: what is not finite before a
+// start stays there.
+__global__ void __launch_bounds__(512) k_delta_carry(const __grid_constant__ mdn_delta c,
+                                                     const __grid_constant__ Segments seg) {
+    __shared__ __align__(16) float now[2][128][16];
+    const uint32_t dk = c.key_dim, dv = c.value_dim, r = threadIdx.x >> 2, e0 = (threadIdx.x & 3) * 4;
+    const uint32_t col = blockIdx.y * 16 + e0, env = blockIdx.x / c.heads, cols = col < dv ? min(4u, dv - col) : 0u;
+    const size_t rows = size_t(c.envs) * c.heads * dk, row = size_t(blockIdx.x) * dk + r;
+    const bool fresh = live_steps(c, env) && c.starts && c.starts[int64_t(env) * c.starts_env];
+    if (r < dk)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++)
+            now[0][r][e0 + e] = c.state_in && !fresh && e < cols ? c.state_in[row * dv + col + e] : 0.0f;
+    for (uint32_t s = 0; s + 1 < seg.count; s++) {
+        const float(*from)[16] = now[s & 1];
+        float* carry = seg.carry + (s * rows + row) * dv + col;
+        const float* map = seg.map + (s * rows + row) * dk;
+        __syncthreads();
+        if (r < dk) {
+            float x[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) x[e] = e < cols ? carry[e] : 0.0f;
+            auto add = [&](float y, uint32_t k) {
+                const uint4 z = *reinterpret_cast<const uint4*>(&from[k][e0]);
+                const uint32_t keep = y != 0.0f ? ~0u : 0u;  // no branch, so that the loads run ahead
+                x[0] = fmaf(y, __uint_as_float(z.x & keep), x[0]);
+                x[1] = fmaf(y, __uint_as_float(z.y & keep), x[1]);
+                x[2] = fmaf(y, __uint_as_float(z.z & keep), x[2]);
+                x[3] = fmaf(y, __uint_as_float(z.w & keep), x[3]);
+            };
+            if (dk % 4 == 0) {
+#pragma unroll 8
+                for (uint32_t k = 0; k < dk; k += 4) {
+                    const float4 y = __ldg(reinterpret_cast<const float4*>(map + k));
+                    add(y.x, k), add(y.y, k + 1), add(y.z, k + 2), add(y.w, k + 3);
+                }
+            } else {
+                for (uint32_t k = 0; k < dk; k++) add(__ldg(map + k), k);
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                now[(s + 1) & 1][r][e0 + e] = x[e];
+                if (e < cols) carry[e] = x[e];
+            }
+        }
     }
 }
 
@@ -1839,8 +1942,39 @@ void tick(const mdn_delta& c, cudaStream_t s) {
     else tick<T, 1>(c, s);
 }
 
+// Segments for a rollout of few environments; one where they fill the device
+// anyway or the axis is short. Both passes take as long as a segment does as
+// long as the joining pass, the larger one, fits on the device at once: 2
+// environments x 8 heads, 4,096 steps of 128 keys and values took 530 us whole,
+// 374 us in nine segments (the joining pass in two waves). A segment has at
+// least eight cells, over which the pipeline's start and the carried state's
+// load are spread.
+Segments segments_of(const mdn_delta& c) {
+    const uint32_t cells = (c.steps + kCell - 1) / kCell;
+    const uint64_t joined = uint64_t(c.envs) * c.heads * (value_blocks(c) + (c.key_dim + 63) / 64);
+    const uint64_t room = 148 * (c.key_dim > 64 || c.dtype == MDN_F32 ? 2 : 3);
+    Segments g{1, cells, kRun, nullptr, nullptr};
+    if (!joined || joined * 3 > room || cells < 32) return g;  // two and three segments gain nothing
+    const uint32_t count = uint32_t(std::min(std::min(room / joined + 1, uint64_t(cells / 8)), uint64_t(32)));
+    g.cells = (cells + count - 1) / count;
+    g.count = (cells + g.cells - 1) / g.cells;
+    return g;
+}
+size_t forward_bytes(const mdn_delta& c) {
+    const size_t rows = size_t(segments_of(c).count - 1) * c.envs * c.heads * c.key_dim;
+    return (rows * c.value_dim + 3) / 4 * 16 + rows * c.key_dim * sizeof(float);
+}
+
+template <class T, int DK, bool SPLIT>
+void launch_rollout(const mdn_delta& c, uint32_t vec, uint32_t items, uint32_t columns, const Segments& g, cudaStream_t s) {
+    static_assert(Forward<T, DK>::kSmem <= 227 * 1024, "shared memory");
+    const uint32_t threads = ((std::min(columns, 64u) + 15) / 16 + 2) * 32;
+    const uint32_t blocks = resident_blocks<k_delta_rollout<T, DK, SPLIT>>(Forward<T, DK>::kSmem, 192);
+    k_delta_rollout<T, DK, SPLIT><<<std::min(items, blocks), threads, Forward<T, DK>::kSmem, s>>>(c, vec, items, g);
+}
+
 template <class T, int DK>
-void rollout(const mdn_delta& c, cudaStream_t s) {
+void rollout(const mdn_delta& c, void* workspace, cudaStream_t s) {
     constexpr uint32_t e = sizeof(T);
     uint32_t vec = 0;
     if (aligned_rows(c.q, e, 16)) vec |= 1;
@@ -1849,10 +1983,23 @@ void rollout(const mdn_delta& c, cudaStream_t s) {
     if (aligned_rows(c.out, e, 2 * e) && c.value_dim % 2 == 0) vec |= 8;
     const uintptr_t states = reinterpret_cast<uintptr_t>(c.state_in) | reinterpret_cast<uintptr_t>(c.state_out);
     if (states % 8 == 0 && c.value_dim % 2 == 0) vec |= 128;
-    static_assert(Forward<T, DK>::kSmem <= 227 * 1024, "shared memory");
-    const uint32_t threads = ((std::min(c.value_dim, 64u) + 15) / 16 + 2) * 32, items = c.envs * c.heads * value_blocks(c);
-    const uint32_t blocks = resident_blocks<k_delta_rollout<T, DK>>(Forward<T, DK>::kSmem, 192);
-    k_delta_rollout<T, DK><<<std::min(items, blocks), threads, Forward<T, DK>::kSmem, s>>>(c, vec, items);
+    const uint32_t rows = c.envs * c.heads;
+    Segments g = segments_of(c);
+    if (!workspace) g = Segments{1, (c.steps + kCell - 1) / kCell, kRun, nullptr, nullptr};
+    if (g.count > 1) {
+        g.carry = static_cast<float*>(workspace);
+        g.map = g.carry + (size_t(g.count - 1) * rows * c.key_dim * c.value_dim + 3) / 4 * 4;
+        g.pass = kJoin;
+        launch_rollout<T, DK, true>(c, vec, (g.count - 1) * rows * (value_blocks(c) + (c.key_dim + 63) / 64),
+                              std::max(c.key_dim, c.value_dim), g, s);
+        cuda_check(cudaGetLastError(), "mdn_delta_forward: segments");
+        k_delta_carry<<<dim3(rows, (c.value_dim + 15) / 16), 512, 0, s>>>(c, g);
+        cuda_check(cudaGetLastError(), "mdn_delta_forward: carried states");
+        g.pass = kRun;
+        launch_rollout<T, DK, true>(c, vec, g.count * rows * value_blocks(c), c.value_dim, g, s);
+    } else {
+        launch_rollout<T, DK, false>(c, vec, rows * value_blocks(c), c.value_dim, g, s);
+    }
 }
 
 template <class T, int DK>
@@ -1886,12 +2033,12 @@ void backward(const mdn_delta& c, const mdn_delta_grads& d, cudaStream_t s) {
 }
 
 template <class T>
-void forward(const mdn_delta& c, cudaStream_t s) {
+void forward(const mdn_delta& c, void* workspace, cudaStream_t s) {
     if (c.steps == 1 && !c.saved) return tick<T>(c, s);
     switch (padded_key(c.key_dim)) {
-        case 32: return rollout<T, 32>(c, s);
-        case 64: return rollout<T, 64>(c, s);
-        default: return rollout<T, 128>(c, s);
+        case 32: return rollout<T, 32>(c, workspace, s);
+        case 64: return rollout<T, 64>(c, workspace, s);
+        default: return rollout<T, 128>(c, workspace, s);
     }
 }
 
@@ -1912,7 +2059,18 @@ extern "C" size_t mdn_delta_workspace_bytes(const mdn_delta* call) {
     return n;
 }
 
+extern "C" size_t mdn_delta_forward_bytes(const mdn_delta* call) {
+    using namespace mdn;
+    size_t n = 0;
+    guarded([&] { check_shape(call, "mdn_delta_forward_bytes"), n = forward_bytes(*call); });
+    return n;
+}
+
 extern "C" int mdn_delta_forward(const mdn_delta* call, void* stream) {
+    return mdn_delta_forward_with(call, nullptr, stream);
+}
+
+extern "C" int mdn_delta_forward_with(const mdn_delta* call, void* workspace, void* stream) {
     using namespace mdn;
     return guarded([&] {
         const char* who = "mdn_delta_forward";
@@ -1923,9 +2081,11 @@ extern "C" int mdn_delta_forward(const mdn_delta* call, void* stream) {
             check_inputs(call, who);
             check_rows(c.out, c.dtype == MDN_F32 ? 4 : 2, who, "out");
         }
+        require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MDN_ERR_INVALID,
+                "mdn_delta_forward: workspace is not 16-byte aligned");
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (c.dtype == MDN_F32) forward<float>(c, s);
-        else forward<bf16>(c, s);
+        if (c.dtype == MDN_F32) forward<float>(c, workspace, s);
+        else forward<bf16>(c, workspace, s);
         cuda_check(cudaGetLastError(), who);
     });
 }

@@ -22,6 +22,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _GATES = {"sigmoid": 0, "silu": 1}
 _NORMALIZE = 1
 MAX_DIM = 128  # MDN_DELTA_MAX_DIM
+_LONG = 32 * 16 - 15  # no shorter rollout is cut into segments (mdn_delta_forward_bytes)
 MAX_NORM_DIM = 8192  # MDN_NORM_MAX_DIM
 
 # mdn_delta, mdn_delta_grads, mdn_block_norm, mdn_block_norm_grads
@@ -164,7 +165,12 @@ def delta_rule(q, k, v, log_decay, beta, state=None, *, starts=None, lengths=Non
         call = _delta_call(*args, 0)
         kept = torch.empty(lib().mdn_delta_saved_bytes(call), dtype=torch.uint8, device=device)
     call = _delta_call(*args, 0 if kept is None else kept.data_ptr())
-    _launch(device, lib().mdn_delta_forward, call)
+    size = lib().mdn_delta_forward_bytes(call) if steps >= _LONG else 0
+    if size:  # few environments, a long axis
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        _launch(device, lib().mdn_delta_forward_with, call, work.data_ptr())
+    else:
+        _launch(device, lib().mdn_delta_forward, call)
     if not save:
         return out, state_out
     saved = DeltaSaved()

@@ -661,3 +661,51 @@ def test_example_learns_and_ticks_agree():
     losses, off = example.run(envs=96, horizon=24, rollouts=5, report=lambda line: None)
     assert losses[-1] < 0.7 * losses[0], losses
     assert max(off) <= 4 * F32_NORM, off
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(20, 700, 1, 1, 16, 16), (18, 400, 1, 2, 24, 72), (7, 500, 1, 1, 100, 40)])
+def test_more_environments_than_fit_at_once(torch, mdn, shape, dtype):
+    """Blocks that go through several environments, some of them without any step."""
+    r = Rollout(torch, dtype, *shape, resets=0.05, ragged=True)
+    want_out, want_state, want = r.exact(grad=True)
+    args = r.gpu(*Rollout.NAMES)
+    starts, lengths, dout, dstate = r.gpu("starts", "lengths", "dout", "dstate")
+    out, state, saved = mdn.delta_rule(*args, starts=starts, lengths=lengths, save=True)
+    close(out, want_out, "out")
+    close(state, want_state, "state")
+    for name, g, w in zip(Rollout.NAMES, mdn.delta_rule_backward(saved, dout, dstate), want):
+        close(g, w, "d" + name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape,resets,ragged", [
+    ((497, 1, 1, 1, 64, 64), 0.0, False), ((512, 3, 1, 2, 32, 48), 0.01, True), ((1030, 2, 2, 2, 40, 72), 0.002, True),
+    ((700, 1, 1, 1, 128, 17), 0.0, False), ((2100, 1, 1, 1, 33, 128), 0.001, False)])
+def test_segments_of_a_long_axis(torch, mdn, shape, resets, ragged, dtype):
+    """Long rollouts of few environments, cut into segments and joined; gradients from the states that were saved."""
+    r = Rollout(torch, dtype, *shape, resets=resets, ragged=ragged, seed=9)
+    want_out, want_state, want = r.exact(grad=True)
+    args = r.gpu(*Rollout.NAMES)
+    starts, lengths, dout, dstate = r.gpu("starts", "lengths", "dout", "dstate")
+    out, state, saved = mdn.delta_rule(*args, starts=starts, lengths=lengths, save=True)
+    close(out, want_out, "out")
+    close(state, want_state, "state")
+    for name, g, w in zip(Rollout.NAMES, mdn.delta_rule_backward(saved, dout, dstate), want):
+        close(g, w, "d" + name)
+
+
+@pytest.mark.parametrize("at", [0, 100, 530])
+def test_segments_keep_episodes_apart(torch, mdn, at):
+    """What is not finite before a start, in the state or the inputs, does not pass a segment's border."""
+    r = Rollout(torch, "f32", 900, 1, 1, 1, 32, 32)
+    r.starts = torch.zeros(900, 1, dtype=torch.uint8)
+    r.starts[at, 0] = 1
+    args = r.gpu(*Rollout.NAMES)
+    clean = mdn.delta_rule(*args, starts=r.starts.cuda())
+    dirty = [x.clone() for x in args]
+    dirty[5][:] = float("nan")
+    for x in dirty[:3]:
+        x[:at] = float("inf")
+    got = mdn.delta_rule(*dirty, starts=r.starts.cuda())
+    assert torch.equal(got[0][at:], clean[0][at:]) and torch.equal(got[1], clean[1])
