@@ -534,7 +534,10 @@ extern "C" int mdn_sim_create(mdn_device* dev, const mdn_sim_config* cfg, const 
                    "upload raptor");
         cuda_check(cudaMemcpyAsync(sim->buf[MDN_BUF_PHYSICS], &params, sizeof(params), cudaMemcpyHostToDevice, sim->stream),
                    "upload physics");
-        for (int id : {MDN_BUF_OBS, MDN_BUF_CO, MDN_BUF_ACTIONS, MDN_BUF_LOGP, MDN_BUF_VALUES, MDN_BUF_REWARDS,
+        // The first reset copies each world and leaves unused obstacle slots as
+        // they are, so that these start at zero too (cudaMalloc clears nothing).
+        for (int id : {MDN_BUF_STATES, MDN_BUF_RUNS, MDN_BUF_WORLDS, MDN_BUF_SENSORS, MDN_BUF_POSES, MDN_BUF_COMMANDS,
+                       MDN_BUF_OBS, MDN_BUF_CO, MDN_BUF_ACTIONS, MDN_BUF_LOGP, MDN_BUF_VALUES, MDN_BUF_REWARDS,
                        MDN_BUF_NEXT_VALUES, MDN_BUF_TERMINATED, MDN_BUF_TRUNCATED, MDN_BUF_ADVANTAGES, MDN_BUF_RETURNS,
                        MDN_BUF_CONTACT_ID, MDN_BUF_TASK_STATES})
             cuda_check(cudaMemsetAsync(sim->buf[id], 0, b[id], sim->stream), "clear rollout buffers");
