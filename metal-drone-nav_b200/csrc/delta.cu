@@ -53,7 +53,10 @@ __device__ __forceinline__ float unit_factor(float x) {
 // thread: column units of V values (V = 4: 16-byte accesses) across lanes, and
 // NI = 32 / V consecutive rows for each of the GT / CP row groups. GT = 32
 // keeps all sums inside a warp; larger states join their warps' sums in shared
-// memory.
+// memory. 65,536 environments x 4 heads of 32 x 32: 423 us, 5.3 TB/s; 8,192 x 4
+// of 64 x 64: 204 us, 5.4 TB/s, of 6.55 TB/s that a copy reaches. Six blocks of
+// 128 an SM hide more latency than five (230 us), at the price of a few spills;
+// GT = 32 is best left to the compiler's 93 registers.
 template <class T, int V, int GT>
 __global__ void __launch_bounds__(GT < 128 ? 128 : GT, V == 4 && GT >= 128 ? 768 / GT : 0) k_delta_tick(const __grid_constant__ mdn_delta c, int log_cp) {
     constexpr int NI = 32 / V, kWarps = GT / 32, kGroups = GT < 128 ? 128 / GT : 1;
@@ -771,9 +774,15 @@ __device__ __forceinline__ void store_two(T* p, bool pair, uint32_t col, uint32_
 }
 
 // A CTA takes 64 value columns of one environment and head after the other; a
-// warp for each 16 of them.
+// warp for each 16 of them. 128 steps of 1,024 environments x 4 heads of 64 x 64
+// in bf16: 315 us, six times the time of its bytes. Twelve warps an SM issue in
+// 40% of the cycles: each chunk is a chain of products and cuts of some 2,800
+// cycles in a warp, and the roles' code (about 30 KB) passes the instruction
+// caches, so what is rarely reached is kept out of line. Two blocks an SM with
+// 168 registers a thread; 112 registers allow no third (four warps a scheduler),
+// and 96, which do, gave 338 us.
 template <class T, int DK, bool SPLIT>
-__global__ void __maxnreg__(DK <= 64 ? 112 : 168) k_delta_rollout(const __grid_constant__ mdn_delta c, uint32_t vec,
+__global__ void __maxnreg__(168) k_delta_rollout(const __grid_constant__ mdn_delta c, uint32_t vec,
                                                                  uint32_t items, const __grid_constant__ Segments seg) {
     using F = Forward<T, DK>;
     constexpr int NP = F::kParts, NT = DK / 8;
@@ -1041,7 +1050,11 @@ __global__ void __launch_bounds__(512) k_delta_carry(const __grid_constant__ mdn
 // Four warps. First each takes 16 value columns (its part of S^T and D^T in
 // registers), then, with D, w and dx in shared memory, 16 of every 64 key
 // columns of dq and dk. A fifth warp prepares the matrices of the next chunk,
-// a sixth fetches the one after.
+// a sixth fetches the one after. 128 steps of 1,024 environments x 4 heads of
+// 64 x 64 in bf16: 1.2 ms, after 0.42 ms for the forward pass that saves the
+// states; 512 environments in 32 bits: 1.4 ms, where the parts of q, k and do
+// leave room for one block an SM. Bound as the forward kernel is, by latency:
+// issue in 32% of the cycles, the tensor cores 22% busy.
 
 template <int N>
 __device__ __forceinline__ void cut_pair(float x, float y, uint32_t (&p)[N]) {
@@ -1868,7 +1881,7 @@ void check_shape(const mdn_delta* c, const char* who) {
             MDN_ERR_INVALID, at + "key_dim and value_dim must be 1..128");
     require(c->dtype == MDN_F32 || c->dtype == MDN_BF16, MDN_ERR_INVALID, at + "dtype must be MDN_F32 or MDN_BF16");
     require((c->flags & ~MDN_DELTA_NORMALIZE) == 0, MDN_ERR_INVALID, at + "unknown flags");
-    require(uint64_t(c->envs) * c->heads <= 0x3fffffffu, MDN_ERR_INVALID, at + "envs x heads exceeds 2^30 - 1");
+    require(uint64_t(c->envs) * c->heads <= 0x7fffffffu, MDN_ERR_INVALID, at + "envs x heads exceeds 2^31 - 1");
     require(c->steps <= 0x7fffffffu, MDN_ERR_INVALID, at + "steps exceeds 2^31 - 1");
 }
 
@@ -1945,14 +1958,14 @@ void tick(const mdn_delta& c, cudaStream_t s) {
 // Segments for a rollout of few environments; one where they fill the device
 // anyway or the axis is short. Both passes take as long as a segment does as
 // long as the joining pass, the larger one, fits on the device at once: 2
-// environments x 8 heads, 4,096 steps of 128 keys and values took 530 us whole,
-// 374 us in nine segments (the joining pass in two waves). A segment has at
+// environments x 8 heads, 4,096 steps of 128 keys and values take 530 us whole,
+// 356 us in five segments, 374 us in nine (the joining pass in two waves). A segment has at
 // least eight cells, over which the pipeline's start and the carried state's
 // load are spread.
 Segments segments_of(const mdn_delta& c) {
     const uint32_t cells = (c.steps + kCell - 1) / kCell;
     const uint64_t joined = uint64_t(c.envs) * c.heads * (value_blocks(c) + (c.key_dim + 63) / 64);
-    const uint64_t room = 148 * (c.key_dim > 64 || c.dtype == MDN_F32 ? 2 : 3);
+    const uint64_t room = 148 * 2;
     Segments g{1, cells, kRun, nullptr, nullptr};
     if (!joined || joined * 3 > room || cells < 32) return g;  // two and three segments gain nothing
     const uint32_t count = uint32_t(std::min(std::min(room / joined + 1, uint64_t(cells / 8)), uint64_t(32)));
