@@ -335,7 +335,9 @@ enum Pass : uint32_t { kRun = 0, kJoin = 1 };
 struct Segments {
     uint32_t count, cells;
     Pass pass;
-    float *carry, *map;  // [count - 1][envs x heads][key][value], [..][key][key]
+    // The state that each segment begins with, [count][envs x heads][key][value] (the first one's is a copy, as the last
+    // segment may write over it), and the maps of all but the last, [count - 1][envs x heads][key][key].
+    float *carry, *map;
 };
 
 __host__ __device__ inline uint32_t value_blocks(const mdn_delta& c) { return (c.value_dim + 63) / 64; }
@@ -836,9 +838,7 @@ __global__ void __maxnreg__(168) k_delta_rollout(const __grid_constant__ mdn_del
         const size_t all = size_t(c.envs) * c.heads * c.key_dim;  // rows of a segment's states
         if (m.flags & (kFirst | kFresh)) {
             const bool unit = SPLIT && m.flags & kMap && !(m.flags & kFresh);
-            const float* from = join || m.flags & kFresh ? nullptr
-                                : segment               ? seg.carry + (segment - 1) * all * dv
-                                                        : c.state_in;
+            const float* from = join || m.flags & kFresh ? nullptr : SPLIT ? seg.carry + segment * all * dv : c.state_in;
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -955,7 +955,7 @@ __global__ void __maxnreg__(168) k_delta_rollout(const __grid_constant__ mdn_del
             uint32_t width = dv;
             if (join) {
                 width = m.flags & kMap ? c.key_dim : dv;
-                to = (m.flags & kMap ? seg.map : seg.carry) + segment * all * width;
+                to = m.flags & kMap ? seg.map + segment * all * width : seg.carry + (segment + 1) * all * width;
             } else {
                 const bool last = !SPLIT || segment + 1 == seg.count;
                 const uint32_t end = last ? c.steps : (segment + 1) * seg.cells * kCell;
@@ -992,11 +992,14 @@ __global__ void __launch_bounds__(512) k_delta_carry(const __grid_constant__ mdn
     const bool fresh = live_steps(c, env) && c.starts && c.starts[int64_t(env) * c.starts_env];
     if (r < dk)
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++)
-            now[0][r][e0 + e] = c.state_in && !fresh && e < cols ? c.state_in[row * dv + col + e] : 0.0f;
+        for (uint32_t e = 0; e < 4; e++) {
+            const float x = c.state_in && !fresh && e < cols ? c.state_in[row * dv + col + e] : 0.0f;
+            now[0][r][e0 + e] = x;
+            if (e < cols) seg.carry[row * dv + col + e] = x;
+        }
     for (uint32_t s = 0; s + 1 < seg.count; s++) {
         const float(*from)[16] = now[s & 1];
-        float* carry = seg.carry + (s * rows + row) * dv + col;
+        float* carry = seg.carry + ((s + 1) * rows + row) * dv + col;
         const float* map = seg.map + (s * rows + row) * dk;
         __syncthreads();
         if (r < dk) {
@@ -1974,8 +1977,8 @@ Segments segments_of(const mdn_delta& c) {
     return g;
 }
 size_t forward_bytes(const mdn_delta& c) {
-    const size_t rows = size_t(segments_of(c).count - 1) * c.envs * c.heads * c.key_dim;
-    return (rows * c.value_dim + 3) / 4 * 16 + rows * c.key_dim * sizeof(float);
+    const size_t count = segments_of(c).count, rows = size_t(c.envs) * c.heads * c.key_dim;
+    return count < 2 ? 0 : (count * rows * c.value_dim + 3) / 4 * 16 + (count - 1) * rows * c.key_dim * sizeof(float);
 }
 
 template <class T, int DK, bool SPLIT>
@@ -2001,7 +2004,7 @@ void rollout(const mdn_delta& c, void* workspace, cudaStream_t s) {
     if (!workspace) g = Segments{1, (c.steps + kCell - 1) / kCell, kRun, nullptr, nullptr};
     if (g.count > 1) {
         g.carry = static_cast<float*>(workspace);
-        g.map = g.carry + (size_t(g.count - 1) * rows * c.key_dim * c.value_dim + 3) / 4 * 4;
+        g.map = g.carry + (size_t(g.count) * rows * c.key_dim * c.value_dim + 3) / 4 * 4;
         g.pass = kJoin;
         launch_rollout<T, DK, true>(c, vec, (g.count - 1) * rows * (value_blocks(c) + (c.key_dim + 63) / 64),
                               std::max(c.key_dim, c.value_dim), g, s);

@@ -709,3 +709,21 @@ def test_segments_keep_episodes_apart(torch, mdn, at):
         x[:at] = float("inf")
     got = mdn.delta_rule(*dirty, starts=r.starts.cuda())
     assert torch.equal(got[0][at:], clean[0][at:]) and torch.equal(got[1], clean[1])
+
+
+def test_segments_with_the_state_in_place(torch, mdn):
+    """state_out may be state_in for a rollout in segments too: the first segment's state is read before the last one
+    writes."""
+    import sys
+    memory = sys.modules[mdn.delta_rule.__module__]
+    r = Rollout(torch, "f32", 1200, 2, 1, 2, 64, 64)
+    q, k, v, g, b, s = r.gpu(*Rollout.NAMES)
+    out, state = mdn.delta_rule(q, k, v, g, b, s)
+    for _ in range(5):
+        place, got = s.clone(), torch.empty_like(out)
+        call = memory._delta_call(q, k, v, g, b, place, None, None, None, True, 1e-6, place, got, 0)
+        size = mdn.lib().mdn_delta_forward_bytes(call)
+        assert size > 0
+        work = torch.empty(size, dtype=torch.uint8, device="cuda")
+        mdn.capi.check(mdn.lib().mdn_delta_forward_with(call, work.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(got, out) and torch.equal(place, state)
