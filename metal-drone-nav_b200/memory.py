@@ -163,11 +163,11 @@ def delta_rule(q, k, v, log_decay, beta, state=None, *, starts=None, lengths=Non
     args = (q, k, v, log_decay, beta, state, starts, lengths, scale, normalize, norm_eps, state_out, out)
     if save:
         call = _delta_call(*args, 0)
-        kept = torch.empty(lib().mdn_delta_saved_bytes(call), dtype=torch.uint8, device=device)
+        kept = q.new_empty(lib().mdn_delta_saved_bytes(call), dtype=torch.uint8)
     call = _delta_call(*args, 0 if kept is None else kept.data_ptr())
     size = lib().mdn_delta_forward_bytes(call) if steps >= _LONG else 0
     if size:  # few environments, a long axis
-        work = torch.empty(size, dtype=torch.uint8, device=device)
+        work = q.new_empty(size, dtype=torch.uint8)
         _launch(device, lib().mdn_delta_forward_with, call, work.data_ptr())
     else:
         _launch(device, lib().mdn_delta_forward, call)
@@ -184,14 +184,14 @@ def delta_rule_backward(saved, dout, dstate=None):
     (dq, dk, dv, dlog_decay, dbeta, dstate) in the shapes and types of q, k, v, log_decay, beta and state."""
     steps, envs, qk, heads, dk, dv = saved.shape
     device, dtype = saved.device, saved.dtype
-    dq = torch.empty((steps, envs, qk, dk), dtype=dtype, device=device)
-    dkey = torch.empty_like(dq)
-    dvalue = torch.empty((steps, envs, heads, dv), dtype=dtype, device=device)
-    dlog_decay = torch.empty((steps, envs, heads), dtype=torch.float32, device=device)
-    dbeta = torch.empty_like(dlog_decay)
-    dstate_in = torch.empty((envs, heads, dk, dv), dtype=torch.float32, device=device)
+    like = saved.tensors[0]
+    dq, dkey = like.new_empty((steps, envs, qk, dk)), like.new_empty((steps, envs, qk, dk))
+    dvalue = like.new_empty((steps, envs, heads, dv))
+    dlog_decay = like.new_empty((steps, envs, heads), dtype=torch.float32)
+    dbeta = like.new_empty((steps, envs, heads), dtype=torch.float32)
+    dstate_in = like.new_empty((envs, heads, dk, dv), dtype=torch.float32)
     size = lib().mdn_delta_workspace_bytes(saved.call)
-    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    work = like.new_empty(size, dtype=torch.uint8) if size else None
     grads = _DELTA_GRADS.pack(
         *_rows(dout, "dout", (steps, envs, heads, dv), dtype, device),
         _plain(dstate, "dstate", (envs, heads, dk, dv), torch.float32, device),
@@ -328,13 +328,14 @@ def block_norm_backward(h, branch=None, gate=None, branch_weight=None, residual_
         _fail("dy must be float32 or bfloat16")
     call = _pack_norm(h if branch is None else None, branch, gate, branch_weight, residual_scale, norm_weight,
                       h if branch is not None else None, None, gate_act, eps, kind, device)
-    dx = torch.empty(shape, dtype=h.dtype, device=device)
-    dbranch = None if branch is None else torch.empty(shape, dtype=kind, device=device)
-    dgate = None if gate is None else torch.empty(shape, dtype=kind, device=device)
-    weights = [torch.empty(shape[1], dtype=torch.float32, device=device) if w is not None and has else None
-               for w, has in ((branch_weight, branch is not None), (residual_scale, branch is not None),
-                              (norm_weight, True))]
-    work = torch.empty(lib().mdn_block_norm_workspace_bytes(call), dtype=torch.uint8, device=device)
+    dx = h.new_empty(shape)
+    dbranch = None if branch is None else branch.new_empty(shape)
+    dgate = None if gate is None else gate.new_empty(shape)
+    rows = h.new_empty((3, shape[1]), dtype=torch.float32).unbind()
+    weights = [row if w is not None and has else None
+               for row, w, has in ((rows[0], branch_weight, branch is not None),
+                                   (rows[1], residual_scale, branch is not None), (rows[2], norm_weight, True))]
+    work = h.new_empty(lib().mdn_block_norm_workspace_bytes(call), dtype=torch.uint8)
     grads = _NORM_GRADS.pack(
         *_matrix(dh, "dh", shape, h.dtype, device), *_matrix(dy, "dy", shape, kind, device), dx.data_ptr(), dx.stride(0),
         *((0, 0) if dbranch is None else (dbranch.data_ptr(), dbranch.stride(0))),
